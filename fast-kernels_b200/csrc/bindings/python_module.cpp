@@ -13,6 +13,7 @@
 
 #include "ops/clustered_page_decode/clustered_page_decode.h"
 #include "ops/decode_quant_linear/arc_w4a16.h"
+#include "ops/paged_kv/paged_kv.h"
 #include "ops/prefix_union_decode/prefix_union_decode.h"
 
 #ifndef FK_COMPILED_WITH_CUDA
@@ -327,6 +328,26 @@ PYBIND11_MODULE(_native, m) {
       py::arg("num_pages"), py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("head_dim"),
       py::arg("page_size"), py::arg("cluster_size"), py::arg("kv_format"), py::arg("keys_are_rotated"),
       py::arg("softmax_scale"), py::arg("rope_theta"), py::arg("stream_ptr"));
+  // ---- what fills the pages --------------------------------------------------------------------
+  m.def(
+      "paged_kv_append_forward",
+      [](ptr_t keys_ptr, ptr_t values_ptr, std::int64_t key_token_stride, std::int64_t key_head_stride,
+         std::int64_t value_token_stride, std::int64_t value_head_stride, ptr_t key_pages_ptr, ptr_t value_pages_ptr,
+         ptr_t key_scales_ptr, ptr_t value_scales_ptr, ptr_t segments_ptr, int num_segments, int num_tokens,
+         int num_pages, int num_kv_heads, int head_dim, int page_size, int kv_format, int rotate_keys,
+         float rope_theta, ptr_t stream_ptr) {
+        py::gil_scoped_release release;
+        fast_kernels::paged_kv::paged_kv_append_forward(
+            keys_ptr, values_ptr, key_token_stride, key_head_stride, value_token_stride, value_head_stride,
+            key_pages_ptr, value_pages_ptr, key_scales_ptr, value_scales_ptr, segments_ptr, num_segments, num_tokens,
+            num_pages, num_kv_heads, head_dim, page_size, kv_format, rotate_keys, rope_theta, stream_ptr);
+      },
+      py::arg("keys_ptr"), py::arg("values_ptr"), py::arg("key_token_stride"), py::arg("key_head_stride"),
+      py::arg("value_token_stride"), py::arg("value_head_stride"), py::arg("key_pages_ptr"),
+      py::arg("value_pages_ptr"), py::arg("key_scales_ptr"), py::arg("value_scales_ptr"), py::arg("segments_ptr"),
+      py::arg("num_segments"), py::arg("num_tokens"), py::arg("num_pages"), py::arg("num_kv_heads"),
+      py::arg("head_dim"), py::arg("page_size"), py::arg("kv_format"), py::arg("rotate_keys"), py::arg("rope_theta"),
+      py::arg("stream_ptr"));
   m.def("page_decode_device_status", []() {
     py::gil_scoped_release release;
     return fast_kernels::clustered_page_decode::page_decode_device_status();

@@ -1,0 +1,47 @@
+// What the paged-KV operators share: page formats, the rotary angle, checks of arguments.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include <cstdint>
+#include <string>
+
+#include "../decode_quant_linear/w4a16_common.cuh"
+#include "fk_paged_kv.h"
+
+namespace fk_paged_kv {
+
+constexpr int kKvBf16 = FK_PAGED_KV_BF16;
+constexpr int kKvFp8 = FK_PAGED_KV_FP8_E4M3;
+constexpr int kKvInt8 = FK_PAGED_KV_INT8;
+constexpr int kScaleBlock = 64;  // dimensions that share a scale
+constexpr int kMaxPairs = 64;
+
+// Turns per position of every rotary pair: theta^(-2i/d) / (2 pi), in fp64. A position times this has
+// the whole turns taken off before anything is rounded to fp32, so the angle's error does not grow
+// with the position (an fp32 product is off by up to 2^-8 radians at position 131072).
+struct RopeTable {
+  double turns[kMaxPairs];
+};
+void fill_rope_table(RopeTable* table, int head_dim, float theta);
+
+__device__ __forceinline__ float2 rope_cos_sin(double turns_per_position, int position) {
+  const double turns = turns_per_position * static_cast<double>(position);
+  const float half_turns = 2.0f * static_cast<float>(turns - rint(turns));
+  float sn, cs;
+  sincospif(half_turns, &sn, &cs);
+  return make_float2(cs, sn);
+}
+
+__device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Host: the thread's last error message, and the codes that go with it.
+int fail(int code, const std::string& message);
+int fail_cuda(const char* what, cudaError_t err);
+
+}  // namespace fk_paged_kv

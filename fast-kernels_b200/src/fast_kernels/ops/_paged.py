@@ -1,0 +1,169 @@
+"""What the operators around the paged cache share: checks of shapes and caches, the descriptor tables
+of a plan on its devices, and plans remembered by their contents."""
+
+from __future__ import annotations
+
+from collections import OrderedDict
+from contextlib import nullcontext
+from typing import Any, Callable
+
+import numpy as np
+
+from fast_kernels.ops.clustered_page_decode import _SCALE_BLOCK, PagedKVCache, _require_layout, _torch
+
+_ROW_ALIGN = 16  # bytes
+_UPLOAD_ALIGN = 128  # int32 words: 512 bytes
+
+
+def require_geometry(*, num_kv_heads: int, head_dim: int, page_size: int, kv_layout: str, num_q_heads: int | None = None) -> str:
+    layout = _require_layout(kv_layout)
+    if num_kv_heads < 1:
+        raise ValueError("num_kv_heads must be >= 1")
+    if num_q_heads is not None and (num_q_heads < 1 or num_q_heads % num_kv_heads != 0):
+        raise ValueError("num_q_heads must be divisible by num_kv_heads")
+    if head_dim not in {64, 128}:
+        raise ValueError("head_dim must be 64 or 128")
+    if page_size not in {16, 32}:
+        raise ValueError("page_size must be 16 or 32")
+    return layout
+
+
+def host_ints(tensor: Any, name: str, ndim: int) -> np.ndarray:
+    torch = _torch()
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if tensor.ndim != ndim:
+        raise ValueError(f"{name} must be {ndim}D")
+    if tensor.is_floating_point() or tensor.is_complex():
+        raise TypeError(f"{name} must hold integers")
+    return tensor.detach().to(device="cpu", dtype=torch.int64).numpy()
+
+
+def table_and_lengths(page_table: Any, **lengths: Any) -> list[np.ndarray]:
+    """The page table and 1D length tensors as int64 arrays, one non-negative length per request."""
+    table = host_ints(page_table, "page_table", 2)
+    out = [table]
+    for name, tensor in lengths.items():
+        values = host_ints(tensor, name, 1)
+        if values.shape[0] != table.shape[0]:
+            raise ValueError(f"{name} must be a 1D tensor with one entry per request")
+        if values.size and int(values.min()) < 0:
+            raise ValueError(f"{name} must not be negative")
+        if values.size and int(values.max()) >= 1 << 31:
+            raise ValueError(f"{name} must fit 32 bits")
+        out.append(values)
+    return out
+
+
+def require_pages(table: np.ndarray, request: np.ndarray, slot: np.ndarray) -> np.ndarray:
+    """Physical pages of (request, logical page) pairs; every one must be in the table."""
+    if slot.size and int(slot.max()) >= table.shape[1]:
+        raise ValueError("page_table has fewer columns than the tokens need")
+    pages = table[request, slot]
+    if pages.size and int(pages.min()) < 0:
+        raise ValueError("page_table has no page for some of the tokens")
+    if pages.size and int(pages.max()) >= 1 << 31:
+        raise ValueError("page_table entries must fit 32 bits")
+    return pages
+
+
+def remembered(plans: OrderedDict, made_from: tuple, build: Callable[[], Any], use_cache: bool, most: int = 256) -> Any:
+    """A plan by the contents that it was made from; the `most` last ones are kept."""
+    if not use_cache:
+        return build()
+    key = tuple((v.shape, v.tobytes()) if isinstance(v, np.ndarray) else v for v in made_from)
+    plan = plans.get(key)
+    if plan is None:
+        plan = plans[key] = build()
+        while len(plans) > most:
+            plans.popitem(last=False)
+    return plan
+
+
+def on_device(kept: dict[int, Any], device: Any, host: dict[str, np.ndarray]) -> dict[str, Any]:
+    """The descriptor tables as int32 tensors on `device`, uploaded once per device in one copy."""
+    torch = _torch()
+    stream = torch.cuda.current_stream(device)
+    entry = kept.get(device.index)
+    if entry is None:
+        parts, sizes = [], []
+        for values in host.values():
+            gap = -values.size % _UPLOAD_ALIGN
+            parts += [np.ascontiguousarray(values, dtype=np.int32).reshape(-1), np.zeros(gap, dtype=np.int32)]
+            sizes += [values.size, gap]
+        block = torch.from_numpy(np.concatenate(parts)).to(device=device)
+        entry = kept[device.index] = (block, dict(zip(host, block.split(sizes)[::2])), stream.cuda_stream)
+    block, tables, home = entry
+    if stream.cuda_stream != home and not torch.cuda.is_current_stream_capturing():
+        block.record_stream(stream)  # the plan may go away before that stream is done with it
+    return tables
+
+
+def check_rows(tensor: Any, *, name: str, shape: tuple[int, ...], device: Any) -> None:
+    """bf16 rows [tokens, heads, head_dim] on `device`: any token and head strides, each row 16-byte aligned."""
+    torch = _torch()
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if tensor.ndim != 3:
+        raise ValueError(f"{name} must be 3D")
+    if tensor.dtype != torch.bfloat16:
+        raise TypeError(f"{name} must have dtype {torch.bfloat16}")
+    if not tensor.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if tensor.device != device:
+        raise ValueError(f"all CUDA tensors must be on the same device: {name}={tensor.device}, key_pages={device}")
+    if tuple(tensor.shape) != shape:
+        raise ValueError(f"{name} must be shaped {list(shape)}, got {list(tensor.shape)}")
+    if tensor.numel() == 0:
+        return
+    if tensor.stride(2) != 1 or tensor.data_ptr() % _ROW_ALIGN or any(
+            tensor.stride(d) % 8 for d in (0, 1) if tensor.shape[d] > 1):
+        raise ValueError(f"{name} must have contiguous rows that start on 16-byte boundaries")
+
+
+def row_strides(tensor: Any) -> tuple[int, int]:
+    """Token and head strides in elements; the stride of a dimension of one entry is never walked."""
+    return tuple(tensor.stride(d) if tensor.shape[d] > 1 else 0 for d in (0, 1))
+
+
+def check_cache(cache: PagedKVCache, plan: Any) -> Any:
+    """The cache's tensors against its own description and the plan's; returns its device."""
+    torch = _torch()
+    for name in ("num_kv_heads", "head_dim", "page_size", "kv_layout"):
+        if getattr(cache, name) != getattr(plan, name):
+            raise ValueError(f"the plan was made for {name}={getattr(plan, name)}, the cache has {getattr(cache, name)}")
+    device = cache.key_pages.device
+    pages = int(cache.key_pages.shape[0])
+    element = {"bf16_kv": torch.bfloat16, "fp8_kv": torch.uint8, "int8_kv": torch.int8}[cache.kv_layout]
+    shape = (pages, cache.num_kv_heads, cache.page_size, cache.head_dim)
+    blocks = cache.head_dim // _SCALE_BLOCK
+    wanted = [("key_pages", cache.key_pages, element, shape), ("value_pages", cache.value_pages, element, shape)]
+    if cache.kv_layout != "bf16_kv":
+        wanted += [("key_scales", cache.key_scales, torch.float32, (*shape[:2], blocks)),
+                   ("value_scales", cache.value_scales, torch.float32, (*shape[:3], blocks))]
+    for name, tensor, dtype, size in wanted:
+        if not isinstance(tensor, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor")
+        if tensor.dtype != dtype:
+            raise TypeError(f"{name} must have dtype {dtype}")
+        if tuple(tensor.shape) != size:
+            raise ValueError(f"{name} must be shaped {list(size)}, got {list(tensor.shape)}")
+        if not tensor.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
+        if tensor.device != device:
+            raise ValueError(f"all CUDA tensors must be on the same device: {name}={tensor.device}, key_pages={device}")
+        if not tensor.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+    if plan.largest_page >= pages:
+        raise ValueError(f"the plan names page {plan.largest_page}, the cache has {pages}")
+    return device
+
+
+def current(device: Any) -> Any:
+    """Makes `device` the current one for a launch, where it is not already."""
+    torch = _torch()
+    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def address(tensor: Any | None) -> int:
+    return 0 if tensor is None else int(tensor.data_ptr())
