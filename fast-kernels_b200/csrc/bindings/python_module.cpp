@@ -328,7 +328,7 @@ PYBIND11_MODULE(_native, m) {
       py::arg("num_pages"), py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("head_dim"),
       py::arg("page_size"), py::arg("cluster_size"), py::arg("kv_format"), py::arg("keys_are_rotated"),
       py::arg("softmax_scale"), py::arg("rope_theta"), py::arg("stream_ptr"));
-  // ---- what fills the pages --------------------------------------------------------------------
+  // ---- what fills the pages, and attention of many rows over them ---------------------------------
   m.def(
       "paged_kv_append_forward",
       [](ptr_t keys_ptr, ptr_t values_ptr, std::int64_t key_token_stride, std::int64_t key_head_stride,
@@ -348,6 +348,61 @@ PYBIND11_MODULE(_native, m) {
       py::arg("num_segments"), py::arg("num_tokens"), py::arg("num_pages"), py::arg("num_kv_heads"),
       py::arg("head_dim"), py::arg("page_size"), py::arg("kv_format"), py::arg("rotate_keys"), py::arg("rope_theta"),
       py::arg("stream_ptr"));
+  m.def(
+      "paged_attention_forward",
+      [](ptr_t query_ptr, std::int64_t query_row_stride, std::int64_t query_head_stride, ptr_t key_ptr, ptr_t
+         value_ptr, ptr_t key_scales_ptr, ptr_t value_scales_ptr, ptr_t page_ids_ptr, ptr_t
+         vectors_ptr, ptr_t items_ptr, ptr_t output_ptr, ptr_t partials_ptr, int num_rows, int
+         num_page_ids, int num_vectors, int num_items, int num_partials, int num_pages, int
+         num_q_heads, int num_kv_heads, int head_dim, int page_size, int kv_format, float
+         softmax_scale, float rope_theta, ptr_t stream_ptr) {
+        py::gil_scoped_release release;
+        fast_kernels::paged_kv::paged_attention_forward(
+            query_ptr, query_row_stride, query_head_stride, key_ptr, value_ptr, key_scales_ptr,
+            value_scales_ptr, page_ids_ptr, vectors_ptr, items_ptr, output_ptr, partials_ptr,
+            num_rows, num_page_ids, num_vectors, num_items, num_partials, num_pages, num_q_heads,
+            num_kv_heads, head_dim, page_size, kv_format, softmax_scale, rope_theta, stream_ptr);
+      },
+      py::arg("query_ptr"), py::arg("query_row_stride"), py::arg("query_head_stride"), py::arg("key_ptr"),
+      py::arg("value_ptr"), py::arg("key_scales_ptr"), py::arg("value_scales_ptr"),
+      py::arg("page_ids_ptr"), py::arg("vectors_ptr"), py::arg("items_ptr"), py::arg("output_ptr"),
+      py::arg("partials_ptr"), py::arg("num_rows"), py::arg("num_page_ids"), py::arg("num_vectors"),
+      py::arg("num_items"), py::arg("num_partials"), py::arg("num_pages"), py::arg("num_q_heads"),
+      py::arg("num_kv_heads"), py::arg("head_dim"), py::arg("page_size"), py::arg("kv_format"),
+      py::arg("softmax_scale"), py::arg("rope_theta"), py::arg("stream_ptr"));
+  m.def(
+      "shared_prefix_decode_forward",
+      [](ptr_t query_ptr, ptr_t key_ptr, ptr_t value_ptr, ptr_t key_scales_ptr, ptr_t value_scales_ptr, ptr_t
+         page_ids_ptr, ptr_t vectors_ptr, ptr_t items_ptr, ptr_t of_request_ptr, ptr_t
+         run_base_pages_ptr, ptr_t run_page_counts_ptr, ptr_t run_logical_starts_ptr, ptr_t
+         run_last_page_lens_ptr, ptr_t request_run_offsets_ptr, ptr_t seq_lens_ptr, ptr_t output_ptr,
+         ptr_t partials_ptr, int batch, int num_page_ids, int num_items, int num_partials, int
+         num_runs, int max_tail_pages, int num_pages, int num_q_heads, int num_kv_heads, int
+         head_dim, int page_size, int kv_format, float softmax_scale, float rope_theta, ptr_t
+         stream_ptr) {
+        py::gil_scoped_release release;
+        fast_kernels::paged_kv::shared_prefix_decode_forward(
+            query_ptr, key_ptr, value_ptr, key_scales_ptr, value_scales_ptr, page_ids_ptr, vectors_ptr,
+            items_ptr, of_request_ptr, run_base_pages_ptr, run_page_counts_ptr,
+            run_logical_starts_ptr, run_last_page_lens_ptr, request_run_offsets_ptr, seq_lens_ptr,
+            output_ptr, partials_ptr, batch, num_page_ids, num_items, num_partials, num_runs,
+            max_tail_pages, num_pages, num_q_heads, num_kv_heads, head_dim, page_size, kv_format,
+            softmax_scale, rope_theta, stream_ptr);
+      },
+      py::arg("query_ptr"), py::arg("key_ptr"), py::arg("value_ptr"), py::arg("key_scales_ptr"),
+      py::arg("value_scales_ptr"), py::arg("page_ids_ptr"), py::arg("vectors_ptr"),
+      py::arg("items_ptr"), py::arg("of_request_ptr"), py::arg("run_base_pages_ptr"),
+      py::arg("run_page_counts_ptr"), py::arg("run_logical_starts_ptr"),
+      py::arg("run_last_page_lens_ptr"), py::arg("request_run_offsets_ptr"), py::arg("seq_lens_ptr"),
+      py::arg("output_ptr"), py::arg("partials_ptr"), py::arg("batch"), py::arg("num_page_ids"),
+      py::arg("num_items"), py::arg("num_partials"), py::arg("num_runs"), py::arg("max_tail_pages"),
+      py::arg("num_pages"), py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("head_dim"),
+      py::arg("page_size"), py::arg("kv_format"), py::arg("softmax_scale"), py::arg("rope_theta"),
+      py::arg("stream_ptr"));
+  m.def("paged_kv_device_status", []() {
+    py::gil_scoped_release release;
+    return fast_kernels::paged_kv::paged_kv_device_status();
+  });
   m.def("page_decode_device_status", []() {
     py::gil_scoped_release release;
     return fast_kernels::clustered_page_decode::page_decode_device_status();

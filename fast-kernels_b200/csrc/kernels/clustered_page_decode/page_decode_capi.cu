@@ -346,31 +346,10 @@ cudaError_t launch_variant(const Variant& v, const DecodeParams& params, int blo
 
 }  // namespace fk_page_decode
 
-using namespace fk_page_decode;
+namespace fk_page_decode {
+namespace {
 
-extern "C" {
-
-FK_PAGE_DECODE_API const char* fk_page_decode_last_error(void) { return t_last_error.c_str(); }
-
-FK_PAGE_DECODE_API size_t fk_page_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim) {
-  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) {
-    fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "workspace_bytes: batch and head counts must be positive, head_dim 64 or 128");
-    return 0;
-  }
-  // the fixed ticket header plus kWorkspaceBlocks partial results of the widest head tile: more
-  // than any automatic plan uses (at most one block per SM shares a task with others)
-  return kTicketBytes + static_cast<size_t>(kWorkspaceBlocks) * partial_floats(8, head_dim) * 4;
-}
-
-FK_PAGE_DECODE_API int fk_page_decode_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
-  if (workspace == nullptr || workspace_bytes < kTicketBytes) {
-    return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "workspace_init: workspace is NULL or smaller than its header");
-  }
-  const cudaError_t err = cudaMemsetAsync(workspace, 0, kTicketBytes, static_cast<cudaStream_t>(stream));
-  return err == cudaSuccess ? FK_PAGE_DECODE_OK : fail_cuda("cudaMemsetAsync", err);
-}
-
-FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args) {
+int forward(const fk_page_decode_args* args, const fk_page_decode_prior* prior) {
   if (args == nullptr) {
     return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "args must not be NULL");
   }
@@ -406,6 +385,10 @@ FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args) {
   params.group_size = a.num_q_heads / a.num_kv_heads;
   params.head_tiles = plan.head_tiles;
   params.page_size = a.page_size;
+  if (prior != nullptr) {
+    params.prior = prior->rows;
+    params.prior_of_request = reinterpret_cast<const int2*>(prior->of_request);
+  }
   params.splits = plan.splits;
   params.stages = plan.stages;
   params.cluster_merge = plan.cluster_merge ? 1 : 0;
@@ -422,6 +405,45 @@ FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args) {
   const cudaError_t err = launch_variant(plan.variant, params, static_cast<int>(blocks), plan.warps, plan.stages,
                                          static_cast<cudaStream_t>(a.stream));
   return err == cudaSuccess ? FK_PAGE_DECODE_OK : fail_cuda("page decode launch", err);
+}
+
+}  // namespace
+}  // namespace fk_page_decode
+
+using namespace fk_page_decode;
+
+extern "C" {
+
+FK_PAGE_DECODE_API const char* fk_page_decode_last_error(void) { return t_last_error.c_str(); }
+
+FK_PAGE_DECODE_API size_t fk_page_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim) {
+  if (batch <= 0 || num_q_heads <= 0 || num_kv_heads <= 0 || (head_dim != 64 && head_dim != 128)) {
+    fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "workspace_bytes: batch and head counts must be positive, head_dim 64 or 128");
+    return 0;
+  }
+  // the fixed ticket header plus kWorkspaceBlocks partial results of the widest head tile: more
+  // than any automatic plan uses (at most one block per SM shares a task with others)
+  return kTicketBytes + static_cast<size_t>(kWorkspaceBlocks) * partial_floats(8, head_dim) * 4;
+}
+
+FK_PAGE_DECODE_API int fk_page_decode_workspace_init(void* workspace, size_t workspace_bytes, void* stream) {
+  if (workspace == nullptr || workspace_bytes < kTicketBytes) {
+    return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "workspace_init: workspace is NULL or smaller than its header");
+  }
+  const cudaError_t err = cudaMemsetAsync(workspace, 0, kTicketBytes, static_cast<cudaStream_t>(stream));
+  return err == cudaSuccess ? FK_PAGE_DECODE_OK : fail_cuda("cudaMemsetAsync", err);
+}
+
+FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args) { return forward(args, nullptr); }
+
+FK_PAGE_DECODE_API int fk_page_decode_forward_merged(const fk_page_decode_args* args, const fk_page_decode_prior* prior) {
+  if (prior == nullptr || prior->rows == nullptr || prior->of_request == nullptr) {
+    return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "prior and its arrays must not be NULL");
+  }
+  if (!aligned16(prior->rows) || (reinterpret_cast<uintptr_t>(prior->of_request) & 7u) != 0) {
+    return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "prior rows must be 16-byte aligned, of_request 8-byte");
+  }
+  return forward(args, prior);
 }
 
 FK_PAGE_DECODE_API int fk_page_decode_device_status(int* status) {

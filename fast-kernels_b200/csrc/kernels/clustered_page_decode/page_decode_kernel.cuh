@@ -88,6 +88,13 @@ struct DecodeParams {
   int splits;
   int stages;
   int early_descriptors;  // the run arrays and seq_lens are not written by the preceding kernel
+  // Results over tokens that are not in the runs, one row of head_dim + 4 floats (weighted values,
+  // maximum, denominator, two unused) per query head: request b adds rows
+  // [prior_of_request[b].x + j] * num_q_heads + q_head, j < prior_of_request[b].y, to its own. The
+  // preceding kernel writes these rows and nothing else that this one reads, so with them the wait
+  // for it comes last. NULL: none.
+  const float* prior;
+  const int2* prior_of_request;
   int cluster_merge;      // the S blocks of a task are one thread-block cluster: merge through shared memory
   float scale_log2e;  // softmax scale times log2(e): the kernel works with exp2
   float inv_freq[kMaxPairs];  // theta^(-2 i / head_dim), rounded once from double
@@ -414,15 +421,17 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
   }
   // Nothing of global memory is read before the previous kernel of the stream has completed --
   // except, if the caller says that kernel does not write them, the request descriptors.
-  if (!p.early_descriptors) {
+  const bool has_prior = p.prior != nullptr;
+  if (!p.early_descriptors && !has_prior) {
     fk_w4a16::pdl_wait_for_prerequisites();
   }
 
   const int query_position = p.seq_lens[request] - 1;
   const int run_begin = p.request_run_offsets[request];
   const int run_end = p.request_run_offsets[request + 1];
-  if (query_position < 0 || run_begin >= run_end) {
-    if (p.early_descriptors) {
+  const int2 prior_rows = has_prior ? p.prior_of_request[request] : make_int2(0, 0);
+  if (query_position < 0 || (run_begin >= run_end && prior_rows.y <= 0)) {
+    if (p.early_descriptors || has_prior) {
       fk_w4a16::pdl_wait_for_prerequisites();
     }
     if (split == 0) {
@@ -563,7 +572,7 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
     const int in_round = max(0, min(CAP, mine - local_base));
 
     // ---- first copies of the round, then the per-block tables while they fly ----
-    if (round == 0 && p.early_descriptors) {
+    if (round == 0 && p.early_descriptors && !has_prior) {
       fk_w4a16::pdl_wait_for_prerequisites();
     }
     if ((PAIRS || lane == 0) && !failed) {
@@ -946,6 +955,11 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
   }
   __syncthreads();
 
+  if (has_prior) {
+    fk_w4a16::pdl_wait_for_prerequisites();  // the rows, and whoever still reads the output's old contents
+  }
+  const int priors = split == 0 ? prior_rows.y : 0;
+  const size_t prior_step = static_cast<size_t>(p.num_q_heads) * ROW;
   float* my_partial = p.partials + (static_cast<size_t>(task) * S + split) * (GT * ROW);
   for (int idx = tid; idx < tile_heads * D; idx += threads) {
     const int h = idx / D;
@@ -954,12 +968,27 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
     for (int w = 0; w < warps; ++w) {
       m_all = fmaxf(m_all, merge_m[w * GT + h]);
     }
+    const float* prior_row = nullptr;
+    if (priors > 0) {
+      prior_row = p.prior + (static_cast<size_t>(prior_rows.x) * p.num_q_heads + first_q_head + h) * ROW;
+#pragma unroll 8
+      for (int j = 0; j < priors; ++j) {
+        m_all = fmaxf(m_all, __ldcg(prior_row + j * prior_step + D));
+      }
+    }
     const float m_ref = m_all == -INFINITY ? 0.0f : m_all;
     float l_all = 0.0f, a_all = 0.0f;
     for (int w = 0; w < warps; ++w) {
       const float weight = exp2f(merge_m[w * GT + h] - m_ref);
       l_all += weight * merge_l[w * GT + h];
       a_all += weight * merge_acc[(w * GT + h) * D + d];
+    }
+#pragma unroll 8
+    for (int j = 0; j < priors; ++j) {
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(prior_row + j * prior_step + D));
+      const float weight = exp2f(ml.x - m_ref);
+      l_all += weight * ml.y;
+      a_all += weight * __ldcg(prior_row + j * prior_step + d);
     }
     if (S == 1) {
       const float y = l_all == 0.0f ? 0.0f : a_all / l_all;

@@ -17,4 +17,14 @@ void paged_kv_append_forward(ptr, ptr, stride, stride, stride, stride, ptr, ptr,
   unavailable();
 }
 
+void paged_attention_forward(ptr, stride, stride, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, int, int, int, int, int,
+                             int, int, int, int, int, int, float, float, ptr) {
+  unavailable();
+}
+void shared_prefix_decode_forward(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr,
+                                  int, int, int, int, int, int, int, int, int, int, int, int, float, float, ptr) {
+  unavailable();
+}
+int paged_kv_device_status() { unavailable(); }
+
 }  // namespace fast_kernels::paged_kv

@@ -20,6 +20,11 @@ from fast_kernels.ops.paged_kv_append import (
     paged_kv_append,
     plan_paged_kv_append,
 )
+from fast_kernels.ops.paged_prompt_attention import (
+    PagedPromptPlan,
+    paged_prompt_attention,
+    plan_paged_prompt_attention,
+)
 from fast_kernels.ops.prefix_union_decode import (
     PrefixUnionDecodePlan,
     cuda_prefix_union_decode_available,
@@ -27,6 +32,11 @@ from fast_kernels.ops.prefix_union_decode import (
     plan_prefix_union_decode,
     prefix_union_decode,
     reference_prefix_union_decode,
+)
+from fast_kernels.ops.shared_prefix_decode import (
+    SharedPrefixDecodePlan,
+    plan_shared_prefix_decode,
+    shared_prefix_decode,
 )
 from fast_kernels.ops.decode_quant_linear import (
     LAYOUT_TO_GROUP_SIZE,
@@ -57,6 +67,12 @@ __all__ = [
     "empty_paged_kv",
     "paged_kv_append",
     "plan_paged_kv_append",
+    "PagedPromptPlan",
+    "paged_prompt_attention",
+    "plan_paged_prompt_attention",
+    "SharedPrefixDecodePlan",
+    "plan_shared_prefix_decode",
+    "shared_prefix_decode",
     "PrefixUnionDecodePlan",
     "cuda_prefix_union_decode_available",
     "estimate_prefix_union_decode_metrics",

@@ -121,6 +121,21 @@ def check_rows(tensor: Any, *, name: str, shape: tuple[int, ...], device: Any) -
         raise ValueError(f"{name} must have contiguous rows that start on 16-byte boundaries")
 
 
+def check_output(tensor: Any, *, shape: tuple[int, ...], device: Any, name: str = "output") -> None:
+    check_rows(tensor, name=name, shape=shape, device=device)
+    if not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def check_turned_keys(cache: PagedKVCache, rope_theta: float) -> None:
+    if not cache.keys_are_rotated:
+        raise ValueError("the cache's keys must be rotated ahead of time")
+    if cache.key_rope_theta is None:
+        raise ValueError("rotated key caches must record key_rope_theta")
+    if float(cache.key_rope_theta) != float(rope_theta):
+        raise ValueError("rope_theta must match the key_rope_theta used to build the cache")
+
+
 def row_strides(tensor: Any) -> tuple[int, int]:
     """Token and head strides in elements; the stride of a dimension of one entry is never walked."""
     return tuple(tensor.stride(d) if tensor.shape[d] > 1 else 0 for d in (0, 1))

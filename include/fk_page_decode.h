@@ -124,6 +124,19 @@ FK_PAGE_DECODE_API int fk_page_decode_workspace_init(void* workspace, size_t wor
 /* Replaces clustered_page_decode_forward (clustered_page_decode.h:16-25). */
 FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args);
 
+/* The same call where some of a request's tokens are not in its runs and another kernel has attended over
+ * them already (fk_paged_kv_attention): request b's result is merged with prior rows
+ *     rows[(of_request[b][0] + j) * num_q_heads + q_head],  j < of_request[b][1]
+ * of head_dim + 4 floats (weighted values, maximum of the logits in units of ln 2, denominator, two
+ * unused). A request may have prior rows and no runs. seq_lens still says where the query sits. The
+ * kernel launched before this one on the stream must be the one that writes the rows; it may write
+ * nothing else that this call reads, and must itself have waited for the kernel before it. */
+typedef struct fk_page_decode_prior {
+  const float* rows;         /* 16-byte aligned */
+  const int32_t* of_request; /* [batch][2], 8-byte aligned */
+} fk_page_decode_prior;
+FK_PAGE_DECODE_API int fk_page_decode_forward_merged(const fk_page_decode_args* args, const fk_page_decode_prior* prior);
+
 /* Reads and clears the device status word of the current device: 0 = fine, 1 = a bounded wait for
  * a page copy gave up (the outputs of that call are not valid; re-initialise the workspace). */
 FK_PAGE_DECODE_API int fk_page_decode_device_status(int* status);

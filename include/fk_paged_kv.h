@@ -78,7 +78,71 @@ typedef struct fk_paged_kv_append_args {
   void* stream;
 } fk_paged_kv_append_args;
 
+/* Attention of query vectors over lists of pages, cut into items by the caller.
+ *
+ * A vector is one token's query: `vectors` holds [num_vectors][4] int32 = row in `query` and `output`,
+ * position, first partial result, number of partial results. An item is a run of vectors and one kv
+ * head over a range of tokens: `items` holds [num_items][8] int32 = first vector, number of vectors,
+ * kv head, entry of `page_ids` that holds token 0, first token (a multiple of page_size), end token,
+ * causal, partial result. Token t lies in page page_ids[entry + t / page_size], slot t % page_size. A
+ * vector of the item sees tokens first .. end - 1, with causal != 0 only those at or before its
+ * position:
+ *     logit_t = softmax_scale * < R(position) q , k_t >,   sum_t softmax(logit)_t * v_t
+ * The keys in the pages carry their rotation already; R turns dimensions 2i and 2i + 1 as in
+ * fk_paged_kv_append. A vector that sees nothing gets zeros. number of vectors *
+ * (num_q_heads / num_kv_heads) is at most FK_PAGED_KV_ITEM_ROWS.
+ *
+ * An item whose partial result is -1 writes its rows of `output` and must be the only one of its
+ * vectors and kv head. Otherwise it leaves, per vector and query head, the weighted values, the
+ * maximum of the logits in units of ln 2 and the denominator at
+ *     partials[(first partial of the vector + partial result of the item) * num_q_heads + q_head]
+ * (rows of head_dim + 4 floats: values, maximum, denominator, two unused). With `combine` != 0 a second
+ * kernel adds the partial results of every vector that has some, in order, into `output`; without it
+ * the caller hands them to fk_page_decode_forward_merged.
+ *
+ * Rounding. Logits, maxima, denominators and weighted values are fp32. The turned query is rounded to
+ * 16 bits once (bf16 pages: bf16; 8-bit pages: fp16 behind an exact power of two), probabilities to
+ * bf16 once, against keys and values as they are stored (8-bit values times their token's scale relative
+ * to the token's larger one: bf16). A non-finite key or value of a token that counts may reach every
+ * vector of an item; what lies behind a request's last token is never used. */
+#define FK_PAGED_KV_ITEM_ROWS 256
+typedef struct fk_paged_kv_attention_args {
+  const void* query; /* bf16 rows [rows][num_q_heads][head_dim], strides below, 16-byte aligned rows */
+  int64_t query_row_stride; /* in elements, multiples of 8 */
+  int64_t query_head_stride;
+  const void* key_pages;
+  const void* value_pages;
+  const float* key_scales;
+  const float* value_scales;
+  const int32_t* page_ids;
+  const int32_t* vectors;
+  const int32_t* items;
+  void* output; /* bf16 [rows][num_q_heads][head_dim], contiguous */
+  float* partials;
+  int32_t num_rows; /* of query and output */
+  int32_t num_page_ids;
+  int32_t num_vectors;
+  int32_t num_items;
+  int32_t num_partials;
+  int32_t num_pages;
+  int32_t num_q_heads;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t page_size;
+  int32_t kv_format;
+  int32_t combine;
+  float softmax_scale;
+  float rope_theta;
+  void* stream;
+} fk_paged_kv_attention_args;
+
 FK_PAGED_KV_API const char* fk_paged_kv_last_error(void);
+
+FK_PAGED_KV_API int fk_paged_kv_attention(const fk_paged_kv_attention_args* args);
+
+/* Reads and clears the device status word of the current device: 0 = fine, 1 = a bounded wait inside a
+ * kernel gave up (the outputs of that call are not valid). */
+FK_PAGED_KV_API int fk_paged_kv_device_status(int* status);
 
 FK_PAGED_KV_API int fk_paged_kv_append(const fk_paged_kv_append_args* args);
 

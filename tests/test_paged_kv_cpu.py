@@ -7,8 +7,10 @@ import importlib
 import re
 from pathlib import Path
 
+import numpy as np
 import pytest
 import torch
+from paged_kv_testlib import attention64, cache_values, fragmented_table, random_cache, rotate64
 
 REPO = Path(__file__).resolve().parent.parent
 ops = importlib.import_module("fast_kernels.ops")
@@ -104,3 +106,172 @@ def test_native_append_checks_its_arguments_before_the_device() -> None:
                             ({"key_token_stride": 12}, "multiples of 8")):
         with pytest.raises(ValueError, match=message):
             call(**{**good, **change})
+
+
+# ---- attention plans: the descriptors, carried out in fp64, give the attention -------------------------------
+
+
+def _run_items(plan, cache, query64, scale):
+    """What the kernels make of a plan's tables: per vector and query head the partial results (values, maximum, denominator)
+    or the finished row, as {row: fp64 [q_heads, dim]}, {partial: ...}."""
+    keys, values = cache_values(cache)
+    ps, group, dim = plan.page_size, plan.num_q_heads // plan.num_kv_heads, plan.head_dim
+    page_ids, vectors = plan.page_ids_cpu, plan.vectors_cpu.tolist()
+    direct, partials = {}, {}
+    for first_vector, count, head, entry, first, end, causal, partial in plan.items_cpu.tolist():
+        assert count * group <= 256 and first % ps == 0 and first < end
+        pages = page_ids[entry : entry + -(-end // ps)].long()
+        k, v = (x[pages, head].reshape(-1, dim)[first:end] for x in (keys, values))
+        for vector in range(first_vector, first_vector + count):
+            row, position, first_partial, partial_count = vectors[vector]
+            seen = max(0, min(end, position + 1) - first) if causal else end - first
+            for q_head in range(head * group, (head + 1) * group):
+                logits = (k[:seen] @ query64[row, q_head]) * scale
+                top = float(logits.max()) if seen else -np.inf
+                weights = torch.exp(logits - top) if seen else logits
+                result = (weights @ v[:seen], top, float(weights.sum()))
+                key = (row, q_head) if partial < 0 else (first_partial + partial, q_head)
+                place = direct if partial < 0 else partials
+                assert key not in place and (partial < 0 or partial < partial_count)
+                place[key] = result
+    return direct, partials
+
+
+def _merge(parts):
+    top = max(m for _, m, _ in parts)
+    if top == -np.inf:
+        return torch.zeros_like(parts[0][0])
+    return sum(o * np.exp(m - top) for o, m, _ in parts) / sum(l * np.exp(m - top) for _, m, l in parts)
+
+
+@pytest.mark.parametrize(("group", "ps", "lens", "new"), [
+    (4, 16, [70, 5, 33], [70, 0, 1]),
+    (1, 32, [700], [300]),
+    (3, 16, [1, 0, 200], [1, 0, 90]),
+    (8, 32, [2100, 40], [3, 40]),
+    (256, 16, [20], [3]),
+])
+def test_prompt_plan_carried_out_in_fp64_is_the_attention(group, ps, lens, new) -> None:
+    heads, dim = 2, 64
+    table, pages = fragmented_table([-(-n // ps) for n in lens], seed=1)
+    cache = random_cache(layout="int8_kv", pages=pages, heads=heads, page_size=ps, dim=dim, table=table, lens=lens, theta=10000.0,
+                         seed=2, device="cpu")
+    plan = ops.plan_paged_prompt_attention(page_table=cache.page_table, seq_lens=cache.seq_lens, query_lens=torch.tensor(new),
+                                           num_q_heads=group * heads, num_kv_heads=heads, head_dim=dim, page_size=ps,
+                                           kv_layout="int8_kv", use_cache=False)
+    rows = [(b, lens[b] - n + i) for b, n in enumerate(new) for i in range(n)]
+    query = torch.randn((len(rows), group * heads, dim), generator=torch.Generator().manual_seed(3)).double()
+    want = attention64(cache, query, rows, 0.125, 10000.0)
+    direct, partials = _run_items(plan, cache, rotate64(query, [p for _, p in rows], 10000.0), 0.125)
+    assert len(partials) == plan.num_partials * group * heads
+    for row, (_, position, first, count) in enumerate(plan.vectors_cpu.tolist()):
+        assert position == rows[row][1]
+        for head in range(group * heads):
+            parts = [partials[first + j, head] for j in range(count)] if count else [direct[row, head]]
+            torch.testing.assert_close(_merge(parts), want[row, head], rtol=1e-10, atol=1e-12)
+
+
+def test_long_ranges_are_cut_and_short_ones_are_not() -> None:
+    def items(length, new, heads):
+        return ops.plan_paged_prompt_attention(
+            page_table=torch.arange(-(-length // 16))[None], seq_lens=torch.tensor([length]), query_lens=torch.tensor([new]),
+            num_q_heads=heads * 4, num_kv_heads=heads, head_dim=128, page_size=16, kv_layout="bf16_kv", use_cache=False)
+
+    assert items(300, 64, 8).num_items == 8 and items(300, 64, 8).num_partials == 0
+    long = items(32768, 64, 8)  # one group of vectors and 8 kv heads: 18 pieces each would be a wave of 144
+    assert 100 <= long.num_items <= 148 and long.num_partials == 64 * long.num_items // 8
+    assert items(8192, 8192, 8).num_partials == 0  # 1024 items without cutting
+
+
+def _shared_case(ps=16, layout="fp8_kv", heads=2, dim=64):
+    """Nine requests, not sorted: five share 160 tokens of which three share 144 more, two share 320 whole (one of them a
+    page boundary's length, one empty tail), one is alone and one is empty."""
+    page = iter(range(1000))
+    take = lambda tokens: [next(page) for _ in range(tokens // ps)]  # noqa: E731
+    system, document, other = take(160), take(144), take(320)
+    tails = {0: 7, 2: 33, 3: 1, 5: 16, 6: 40, 7: 0, 8: 5}
+    rows = {0: system, 2: system + document, 3: system + document, 5: system, 6: system + document, 7: other, 8: other}
+    lens = [0] * 9
+    for b, prefix in rows.items():
+        lens[b] = len(prefix) * ps + tails[b]
+        rows[b] = prefix + take(-(-tails[b] // ps) * ps)
+    rows[4], lens[4] = take(96), 90
+    rows[1] = []
+    table = np.full((9, max(map(len, rows.values()))), -1, dtype=np.int32)
+    for b, pages in rows.items():
+        table[b, : len(pages)] = pages
+    total = next(page)
+    table[table >= 0] = np.random.RandomState(0).permutation(total)[table[table >= 0]]
+    return random_cache(layout=layout, pages=total, heads=heads, page_size=ps, dim=dim, table=table, lens=lens, theta=10000.0, seed=2,
+                        device="cpu")
+
+
+def _shared_plan(cache, group, **kwargs):
+    return ops.plan_shared_prefix_decode(page_table=cache.page_table, seq_lens=cache.seq_lens, num_q_heads=group * cache.num_kv_heads,
+                                         num_kv_heads=cache.num_kv_heads, head_dim=cache.head_dim, page_size=cache.page_size,
+                                         kv_layout=cache.kv_layout, **{"use_cache": False, "min_saved_bytes": 0, **kwargs})
+
+
+@pytest.mark.parametrize("group", [1, 3, 100])
+def test_shared_plan_carried_out_in_fp64_is_the_attention(group) -> None:
+    cache = _shared_case()
+    plan = _shared_plan(cache, group)
+    assert sorted((first, end, tuple(sorted(who))) for first, end, who in plan.runs) == [
+        (0, 10, (0, 2, 3, 5, 6)), (0, 20, (7, 8)), (10, 19, (2, 3, 6))]
+    lens = cache.seq_lens.tolist()
+    query = torch.randn((9, group * 2, 64), generator=torch.Generator().manual_seed(3)).double()
+    rows = [(b, lens[b] - 1) for b in range(9)]
+    want = attention64(cache, query, rows, 0.125, 10000.0)
+    turned = rotate64(query, [max(0, n - 1) for n in lens], 10000.0)
+    direct, partials = _run_items(plan, cache, turned, 0.125)
+    assert not direct and len(partials) == plan.num_partials * group * 2
+    keys, values = cache_values(cache)
+    tail = plan.tail_plan
+    assert tail.seq_lens_cpu.tolist() == lens
+    offsets = tail.request_run_offsets_cpu.tolist()
+    for b, (first, count) in enumerate(plan.of_request_cpu.tolist()):
+        slots = []
+        for run in range(offsets[b], offsets[b + 1]):
+            base, pages, last = (int(getattr(tail, f"run_{n}_cpu")[run]) for n in ("base_pages", "page_counts", "last_page_lens"))
+            slots += [(base + i, s) for i in range(pages) for s in range(last if i == pages - 1 else 16)]
+        for head in range(group * 2):
+            parts = [partials[first + j, head] for j in range(count)]
+            if slots:
+                k, v = (torch.stack([x[page, head // group, slot] for page, slot in slots]) for x in (keys, values))
+                logits = (k @ turned[b, head]) * 0.125
+                weights = torch.exp(logits - logits.max())
+                parts.append((weights @ v, float(logits.max()), float(weights.sum())))
+            got = _merge(parts) if parts else torch.zeros(64, dtype=torch.float64)
+            torch.testing.assert_close(got, want[b, head], rtol=1e-10, atol=1e-12)
+
+
+def test_shared_plan_without_enough_to_save_is_the_plain_decode() -> None:
+    cache = _shared_case()
+    plan = _shared_plan(cache, 2, min_saved_bytes=1 << 30)
+    assert plan.runs == [] and plan.num_items == 0 and plan.num_partials == 0 and plan.estimated_saved_hbm_bytes == 0
+    plain = ops.plan_clustered_page_decode(page_table=cache.page_table, seq_lens=cache.seq_lens, num_q_heads=4, num_kv_heads=2, head_dim=64,
+                                           page_size=16, kv_layout="fp8_kv", use_cache=False)
+    for name in ("run_base_pages", "run_page_counts", "run_last_page_lens", "request_run_offsets", "seq_lens"):
+        assert torch.equal(getattr(plan.tail_plan, f"{name}_cpu"), getattr(plain, f"{name}_cpu")), name
+    assert plan.tail_plan.max_pages == plain.max_pages
+    assert _shared_plan(cache, 2).estimated_saved_hbm_bytes == (4 * 10 + 2 * 9 + 20) * 2 * (2 * 16 * 64 + 4 * 17)
+
+
+def test_attention_plan_refusals() -> None:
+    arguments = dict(page_table=torch.tensor([[0, 1]]), seq_lens=torch.tensor([20]), query_lens=torch.tensor([3]), num_q_heads=4,
+                     num_kv_heads=2, head_dim=64, page_size=16, kv_layout="bf16_kv", use_cache=False)
+    plan = ops.plan_paged_prompt_attention
+    assert plan(**arguments).num_tokens == 3
+    for change, message in (({"query_lens": torch.tensor([21])}, "must not exceed"), ({"query_lens": torch.tensor([-1])}, "negative"),
+                            ({"num_q_heads": 3}, "divisible"), ({"num_q_heads": 1024}, "at most 256"), ({"head_dim": 32}, "head_dim"),
+                            ({"page_table": torch.tensor([[0, -1]])}, "no page"), ({"page_table": torch.tensor([[0]])}, "fewer columns")):
+        with pytest.raises(ValueError, match=message):
+            plan(**{**arguments, **change})
+    arguments.pop("query_lens")
+    plan = ops.plan_shared_prefix_decode
+    assert plan(**arguments).batch == 1
+    for change, message in (({"min_saved_bytes": -1}, "negative"), ({"num_q_heads": 3}, "divisible"),
+                            ({"page_table": torch.tensor([[0, -1]])}, "no page"), ({"page_table": torch.tensor([[0]])}, "fewer columns"),
+                            ({"page_table": torch.zeros((0, 2), dtype=torch.int32), "seq_lens": torch.zeros(0, dtype=torch.int32)}, "empty")):
+        with pytest.raises(ValueError, match=message):
+            plan(**{**arguments, **change})
