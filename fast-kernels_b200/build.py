@@ -105,7 +105,8 @@ def build_paged_kv_library(force: bool = False) -> Path:
     kernel_dir = CSRC / "kernels" / "paged_kv"
     sources = sorted(kernel_dir.glob("*.cu"))
     deps = (sources + sorted(kernel_dir.glob("*.cuh")) + sorted(kernel_dir.glob("*.h")) + sorted(kernel_dir.glob("*.inc"))
-            + [REPO / "include" / "fk_paged_kv.h", CSRC / "kernels" / "decode_quant_linear" / "w4a16_common.cuh"])
+            + [REPO / "include" / "fk_paged_kv.h"] + sorted((CSRC / "kernels" / "decode_quant_linear").glob("*.cuh"))
+            + sorted((CSRC / "kernels" / "clustered_page_decode").glob("*.cuh")))
     target = LIB_DIR / "libfk_paged_kv.so"
     if not force and _newer(target, deps):
         return target

@@ -40,22 +40,30 @@ int status_word(int** out) {
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-template <int D>
-cudaError_t launch(const AttentionParams& params, int kv_format, int num_items, bool combine, cudaStream_t stream) {
-  if (num_items > 0) {
-    if (kv_format == kKvBf16) {
-      paged_attention_rows_kernel<D, kKvBf16><<<num_items, 256, 0, stream>>>(params);
-    } else if (kv_format == kKvFp8) {
-      paged_attention_rows_kernel<D, kKvFp8><<<num_items, 256, 0, stream>>>(params);
-    } else {
-      paged_attention_rows_kernel<D, kKvInt8><<<num_items, 256, 0, stream>>>(params);
-    }
+cudaError_t launch_items(const AttentionParams& params, int head_dim, int kv_format, int num_items, cudaStream_t stream) {
+  if (head_dim == 64) {
+    return kv_format == kKvBf16 ? launch_attention_d64_bf16(params, num_items, stream)
+           : kv_format == kKvFp8 ? launch_attention_d64_fp8(params, num_items, stream)
+                                 : launch_attention_d64_int8(params, num_items, stream);
   }
-  if (combine && params.num_partials > 0) {
-    const long long warps = static_cast<long long>(params.num_vectors) * params.num_q_heads;
-    combine_partials_kernel<D><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, stream>>>(params);
-  }
-  return cudaGetLastError();
+  return kv_format == kKvBf16 ? launch_attention_d128_bf16(params, num_items, stream)
+         : kv_format == kKvFp8 ? launch_attention_d128_fp8(params, num_items, stream)
+                               : launch_attention_d128_int8(params, num_items, stream);
+}
+
+cudaError_t launch_combine(const AttentionParams& params, int head_dim, cudaStream_t stream) {
+  cudaLaunchConfig_t config{};
+  const long long warps = static_cast<long long>(params.num_vectors) * params.num_q_heads;
+  config.gridDim = dim3(static_cast<unsigned>((warps + 7) / 8), 1, 1);
+  config.blockDim = dim3(256, 1, 1);
+  config.stream = stream;
+  cudaLaunchAttribute attribute{};
+  attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attribute.val.programmaticStreamSerializationAllowed = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  return head_dim == 64 ? cudaLaunchKernelEx(&config, combine_partials_kernel<64>, params)
+                        : cudaLaunchKernelEx(&config, combine_partials_kernel<128>, params);
 }
 
 }  // namespace
@@ -98,6 +106,12 @@ FK_PAGED_KV_API int fk_paged_kv_attention(const fk_paged_kv_attention_args* args
   if (a.query == nullptr || a.key_pages == nullptr || a.value_pages == nullptr || a.page_ids == nullptr ||
       a.vectors == nullptr || a.items == nullptr || a.output == nullptr) {
     return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT, "query, pages, page_ids, vectors, items and output must not be NULL");
+  }
+  if (a.num_pages == 0 || static_cast<long long>(a.num_pages) * a.num_kv_heads * a.page_size > 0x7fffffffLL) {
+    return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT, "num_pages * num_kv_heads * page_size must be positive and fit 31 bits");
+  }
+  if (static_cast<long long>(a.num_vectors) * a.num_q_heads > 0x7fffffffLL) {
+    return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT, "num_vectors * num_q_heads must fit 31 bits");
   }
   if (a.num_partials > 0 && a.partials == nullptr) {
     return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT, "partials must not be NULL when num_partials > 0");
@@ -142,8 +156,10 @@ FK_PAGED_KV_API int fk_paged_kv_attention(const fk_paged_kv_attention_args* args
   params.scale_log2e = static_cast<float>(static_cast<double>(a.softmax_scale) * 1.4426950408889634);
   fill_rope_table(&params.rope, a.head_dim, a.rope_theta);
   const cudaStream_t stream = static_cast<cudaStream_t>(a.stream);
-  const cudaError_t err = a.head_dim == 64 ? launch<64>(params, a.kv_format, a.num_items, a.combine != 0, stream)
-                                           : launch<128>(params, a.kv_format, a.num_items, a.combine != 0, stream);
+  cudaError_t err = launch_items(params, a.head_dim, a.kv_format, a.num_items, stream);
+  if (err == cudaSuccess && a.combine != 0 && a.num_partials > 0) {
+    err = launch_combine(params, a.head_dim, stream);
+  }
   return err == cudaSuccess ? FK_PAGED_KV_OK : fail_cuda("paged attention launch", err);
 }
 

@@ -1,0 +1,827 @@
+// Attention of up to 256 query rows of one kv head over a list of pages, on the fifth-generation
+// tensor cores: both products as tcgen05.mma with the logits, the probabilities and the weighted
+// values in tensor memory.
+//
+// One block per item. Its rows (vectors x query heads of the kv head) are two tiles, X = 0 and 1, of
+// 128 rows; tokens come in tiles of 128. Per token tile j:
+//     S_X = Q_X K_j^T          128 x 128, fp32, tensor memory     (A, B from shared memory)
+//     P_X = 2^(S_X - m_X)      bf16, over S_X's own columns       (one thread per row)
+//     O_X += P_X V_j           128 x head_dim, fp32               (A from tensor memory, B from shared memory)
+// While the softmax warps of one row tile work, the tensor core multiplies for the other. The softmax
+// scale times log2(e) rides on the query, so the exponential is one ex2.
+//
+// The running maximum is kept lazily: O is multiplied by 2^(old - new) only when a row's maximum has
+// grown by more than 2^8 since the last time, else P may be up to 2^8 and nothing is lost (bf16 and
+// fp32 have the range). The tensor core is done with O whenever a tile's logits are: their commit
+// follows the previous tile's second product.
+//
+// Roles (warps): 0-3 and 4-7 softmax of the two row tiles (they also turn and store the queries, and
+// write the results), 8 issues the MMAs, 9 the copies, 10 clears the value rows behind the end (a
+// probability of 0 times whatever a page holds there would not be 0). 8-bit pages: 12-15 convert.
+// Every wait is bounded.
+//
+// Operands in shared memory are rows of 128 bytes (64 16-bit elements) under the 128-byte swizzle; a
+// tile of 128-dimensional rows is two such halves. bf16 pages are copied there by TMA, one box of
+// page_size rows per page and half. 8-bit pages are copied as they are and converted by four warps:
+// keys to fp16, exact for the 64-dim block with the page's larger scale, the other block times the
+// ratio of the two scales; values to bf16 likewise per token. The larger scales stay fp32: the page's
+// goes on the logits, the token's on the probability before it is rounded.
+#pragma once
+
+#include <cuda.h>
+
+#include "../clustered_page_decode/page_decode_kernel.cuh"
+#include "../decode_quant_linear/w4a16_gemm_tile.cuh"
+#include "paged_attention.cuh"
+
+namespace fk_paged_kv {
+
+namespace umma = fk_w4a16::umma;
+namespace tile = fk_w4a16::tile;
+using fk_w4a16::lds64;
+using fk_w4a16::mbar_expect_tx;
+using fk_w4a16::mbar_init;
+using fk_w4a16::mbar_init_fence;
+using fk_w4a16::mbar_wait_parked;
+using fk_w4a16::proxy_fence_async;
+using fk_w4a16::smem_addr;
+
+constexpr int kTileRows = 128;
+constexpr int kTileTokens = 128;
+constexpr int kFactorRing = 4;  // token tiles whose scales are kept for the softmax warps
+constexpr float kLazyGrowth = 8.0f;
+constexpr int kStatusWaitTimeout = 1;
+
+template <int D, int KV>
+struct TcLayout {
+  static constexpr bool kQuant = KV != kKvBf16;
+  static constexpr int kHalves = D / 64;
+  static constexpr int kHalfBytes = kTileTokens * 128;             // 64 dimensions of 128 rows
+  static constexpr int kOperandBytes = kHalves * kHalfBytes;       // a tile of queries, keys or values
+  static constexpr int kSlots = D == 64 ? (kQuant ? 4 : 8) : (kQuant ? 3 : 5);
+  static constexpr int kRawBytes = kTileTokens * D;                // a tile of 8-bit keys or values
+  static constexpr int kRawScaleBytes = kTileTokens * (D / 64) * 4;
+  static constexpr int kRawSlots = kQuant ? (D == 64 ? 6 : 3) : 0;
+  static constexpr int kRawSlotBytes = kRawBytes + kRawScaleBytes;
+  static constexpr int kThreads = kQuant ? 512 : 384;
+  // A softmax thread holds a row of 128 logits. Two warpgroups of them and one or two of the others draw
+  // on what the block was launched with: 2 x 208 + 88 = 3 x 168, 2 x 184 + 2 x 72 = 4 x 128.
+  static constexpr int kSoftmaxRegisters = kQuant ? 184 : 208;
+  static constexpr int kOtherRegisters = kQuant ? 72 : 88;
+  // offsets from a 1024-byte aligned base
+  static constexpr int kQueries = 0;
+  static constexpr int kRing = kQueries + 2 * kOperandBytes;
+  static constexpr int kRaw = kRing + kSlots * kOperandBytes;
+  static constexpr int kKeyFactors = kRaw + kRawSlots * kRawSlotBytes;              // [ring][8 pages]
+  static constexpr int kValueFactors = kKeyFactors + (kQuant ? kFactorRing * 32 : 0);  // [ring][128 tokens]
+  static constexpr int kRawKeyScales = kValueFactors + (kQuant ? kFactorRing * 512 : 0);  // [raw slot][8 pages][2]
+  static constexpr int kRowPower = kRawKeyScales + kRawSlots * 64;                  // [256]
+  static constexpr int kBarriers = kRowPower + (kQuant ? 1024 : 0);
+  static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
+};
+
+__device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+      "}\n" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+// Operand descriptors: 128-byte swizzle (bits 61-63 = 2), version 1 (bit 46), offsets in 16-byte units.
+// Rows are the M or N dimension (K contiguous): groups of 8 rows are 1024 bytes apart.
+__device__ __forceinline__ uint64_t rows_desc(uint32_t address) {
+  return static_cast<uint64_t>((address & 0x3FFFFu) >> 4) | (uint64_t{1} << 16) | (uint64_t{1024 >> 4} << 32) |
+         (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+// Rows are the K dimension (N contiguous): blocks of 64 columns are a half apart, groups of 8 rows 1024 bytes.
+__device__ __forceinline__ uint64_t columns_desc(uint32_t address) {
+  return static_cast<uint64_t>((address & 0x3FFFFu) >> 4) | (uint64_t{(kTileTokens * 128) >> 4} << 16) |
+         (uint64_t{1024 >> 4} << 32) | (uint64_t{1} << 46) | (uint64_t{2} << 61);
+}
+// fp32 accumulate, M = 128; `columns_b`: B's N dimension is contiguous.
+__host__ __device__ constexpr uint32_t instruction_desc(bool bf16, int n, bool columns_b) {
+  return (1u << 4) | ((bf16 ? 1u : 0u) << 7) | ((bf16 ? 1u : 0u) << 10) | ((columns_b ? 1u : 0u) << 16) |
+         (static_cast<uint32_t>(n / 8) << 17) | (static_cast<uint32_t>(kTileRows / 16) << 24);
+}
+// Element (row, 16-byte chunk of the row) of a swizzled operand.
+__device__ __forceinline__ uint32_t operand_chunk(int row, int chunk) {
+  return (chunk >> 3) * (kTileRows * 128) + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+}
+__device__ __forceinline__ void sts128(uint32_t addr, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void st32_tmem(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// Four 8-bit numbers as floats, exactly (e4m3: times 2^-8 where SHIFTED words were asked for).
+template <int KV>
+__device__ __forceinline__ void bytes_to_float4(uint32_t w, float (&x)[4]) {
+  if constexpr (KV == kKvInt8) {
+    const uint32_t u = w ^ 0x80808080u;  // byte + 128 dropped into the mantissa of 2^23
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540u + i)) - 8388736.0f;
+    }
+  } else {
+    uint32_t a, b;
+    fk_page_decode::bytes_to_half2<fk_page_decode::kKvFp8, false>(w, a, b);
+    const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&a));
+    const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&b));
+    x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+  }
+}
+
+template <int D, int KV>
+__global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
+    paged_attention_tc_kernel(const __grid_constant__ AttentionParams p, const __grid_constant__ CUtensorMap key_map,
+                              const __grid_constant__ CUtensorMap value_map) {
+  using L = TcLayout<D, KV>;
+  constexpr bool QUANT = L::kQuant;
+  constexpr int kBlocks = D / 64;          // scale blocks, and halves of an operand
+  constexpr int kChunks = D / 8;           // 16-byte chunks of a row
+  constexpr uint32_t kScoresDesc = instruction_desc(!QUANT, kTileTokens, false);
+  constexpr uint32_t kValuesDesc = instruction_desc(true, D, true);
+  extern __shared__ __align__(16) uint8_t raw_smem[];
+
+  const int tid = static_cast<int>(threadIdx.x);
+  const int lane = tid & 31;
+  const int warp = tid >> 5;
+  const uint32_t base = (smem_addr(raw_smem) + 1023u) & ~1023u;
+  uint8_t* smem = raw_smem + (base - smem_addr(raw_smem));
+  const uint32_t bars = base + L::kBarriers;
+  const uint32_t q_ready = bars + 16;
+  const uint32_t s_ready = bars + 24;             // [2] logits of a tile are there
+  const uint32_t p_ready = bars + 40;             // [2] probabilities are stored (and O is rescaled)
+  const uint32_t o_final = bars + 56;             // [2] the last product is done
+  const uint32_t v_clear = bars + 72;
+  const uint32_t drain = bars + 80;
+  const uint32_t v_landed = bars + 88;
+  const uint32_t full = bars + 96;                // [slots] operand tile is there
+  const uint32_t empty = full + 8 * 8;            // [slots] MMAs are done with it
+  const uint32_t raw_full = empty + 8 * 8;        // [raw slots]
+  const uint32_t raw_empty = raw_full + 8 * 8;
+  volatile uint32_t* fail_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kBarriers + 8);
+  volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kBarriers);
+
+  if (tid == 0) {
+    *fail_flag = 0u;
+    mbar_init(q_ready, 8);
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(s_ready + 8 * x, 1);
+      mbar_init(p_ready + 8 * x, 4);
+      mbar_init(o_final + 8 * x, 1);
+    }
+    mbar_init(v_landed, 1);
+    mbar_init(v_clear, 1);
+    mbar_init(drain, 1);
+    for (int s = 0; s < L::kSlots; ++s) {
+      mbar_init(full + 8 * s, QUANT ? 4 : 1);
+      mbar_init(empty + 8 * s, 1);
+    }
+    for (int s = 0; s < L::kRawSlots; ++s) {
+      mbar_init(raw_full + 8 * s, 1);
+      mbar_init(raw_empty + 8 * s, 4);
+    }
+    mbar_init_fence();
+  }
+  if (warp == 8) {
+    umma::tmem_alloc(bars, 512);
+    umma::tmem_relinquish();
+  }
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  const uint32_t tmem = *tmem_slot;
+
+  // From here on memory is read; the next kernel of the stream may be scheduled, knowing that what was
+  // launched before this one has completed.
+  fk_w4a16::pdl_wait_for_prerequisites();
+  fk_w4a16::pdl_launch_dependents();
+
+  const Item item = load_item(p, blockIdx.x);
+  const bool fits = item_fits(p, item);
+  const int rows = item.vectors * p.group;
+  // Tokens that the rows of tile x see, and how many tiles of them.
+  auto limit_of = [&](int x, bool last) -> int {
+    const int row = last ? min(rows, (x + 1) * kTileRows) - 1 : x * kTileRows;
+    return item.causal != 0 ? min(item.end_token, p.vectors[item.first_vector + row / p.group].y + 1) : item.end_token;
+  };
+  int tiles[2] = {0, 0};
+  int unmasked[2] = {0, 0};  // tokens that every row of the tile sees
+  if (fits) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      if (x * kTileRows < rows) {
+        const int seen = max(0, limit_of(x, true) - item.first_token);
+        tiles[x] = (seen + kTileTokens - 1) / kTileTokens;
+        // positions of an item's vectors need not ascend without `causal`; with it they do
+        unmasked[x] = max(0, limit_of(x, false) - item.first_token);
+      }
+    }
+  }
+  const int count = max(tiles[0], tiles[1]);
+  const int loaded = min(item.end_token - item.first_token, count * kTileTokens);  // tokens that are fetched
+  const bool clear_needed = count > 0 && loaded < count * kTileTokens;
+
+  auto give_up = [&]() {
+    *fail_flag = 1u;
+    atomicExch(p.status, kStatusWaitTimeout);
+  };
+
+  if (warp < 8) {
+    tile::registers_up<L::kSoftmaxRegisters>();
+    const int x = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;      // of the tile; also its tensor memory lane
+    float* row_power = reinterpret_cast<float*>(smem + L::kRowPower);
+    // ---- queries: turned, scaled, rounded, stored ----------------------------------------------
+    if (count > 0) {
+      // A thread takes 8 dimensions (four rotary pairs) of a vector: their cosines and sines serve all
+      // the query heads that it walks. `slices` threads share a vector's heads where there are few vectors.
+      const int columns = item.vectors * kChunks;
+      const int slices = max(1, min(p.group, 256 / columns));
+      const int tasks = columns * slices;
+      const int round = (tasks + 31) / 32 * 32;
+      const int heads_each = (p.group + slices - 1) / slices;
+      for (int task = tid; task < round; task += 256) {
+        const bool active = task < tasks;
+        const int chunk = task % kChunks;
+        const int vector = active ? (task / kChunks) % item.vectors : 0;
+        const int slice = active ? task / columns : 0;
+        const int4 v = p.vectors[item.first_vector + vector];
+        const bool readable = active && v.x >= 0 && v.x < p.num_rows;
+        float2 cs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 turn = rope_cos_sin(p.rope.turns[chunk * 4 + i], v.y);
+          cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
+        }
+        const uint16_t* src = p.query + static_cast<long long>(readable ? v.x : 0) * p.query_row_stride + chunk * 8;
+        for (int h = 0; h < heads_each; ++h) {
+          const int head = slice * heads_each + h;
+          const bool store = active && head < p.group;
+          uint4 w = make_uint4(0u, 0u, 0u, 0u);
+          if (store && readable) {
+            w = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(item.kv_head * p.group + head) *
+                                                              p.query_head_stride));
+          }
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+          float q[8];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float even = bf16_low(words[i]), odd = bf16_high(words[i]);
+            q[2 * i] = even * cs[i].x - odd * cs[i].y;
+            q[2 * i + 1] = even * cs[i].y + odd * cs[i].x;
+          }
+          const int r = vector * p.group + head;
+          uint4 out;
+          if constexpr (QUANT) {
+            // fp16 has the precision but not the range: the row is divided by the power of two of its
+            // largest element, which goes back on in fp32
+            float largest = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              largest = fmaxf(largest, fabsf(q[i]));
+            }
+#pragma unroll
+            for (int o = 1; o < kChunks; o <<= 1) {
+              largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+            }
+            const int bits = fk_page_decode::exponent_bits(largest);
+            const float shrink = fk_page_decode::inverse_power(bits);
+            out = make_uint4(pack_half(q[0] * shrink, q[1] * shrink), pack_half(q[2] * shrink, q[3] * shrink),
+                             pack_half(q[4] * shrink, q[5] * shrink), pack_half(q[6] * shrink, q[7] * shrink));
+            if (store && chunk == 0) {
+              row_power[r] = __int_as_float(bits);
+            }
+          } else {
+            out = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
+          }
+          if (store) {
+            sts128(base + L::kQueries + (r >> 7) * L::kOperandBytes + operand_chunk(r & 127, chunk), out);
+          }
+        }
+      }
+      for (int idx = tid; idx < (256 - rows) * kChunks; idx += 256) {  // rows without a vector
+        const int r = rows + idx / kChunks;
+        sts128(base + L::kQueries + (r >> 7) * L::kOperandBytes + operand_chunk(r & 127, idx % kChunks),
+               make_uint4(0u, 0u, 0u, 0u));
+        if (QUANT && idx % kChunks == 0) {
+          row_power[r] = 0.0f;
+        }
+      }
+      proxy_fence_async();
+      __syncwarp();
+      if (lane == 0) {
+        umma::mbar_arrive(q_ready);
+      }
+      asm volatile("bar.sync 1, 256;" ::: "memory");  // row_power is read by other warps than its writers
+    }
+    // ---- softmax --------------------------------------------------------------------------------
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem + lanes + x * kTileTokens;
+    const uint32_t o_tmem = tmem + lanes + 256 + x * D;
+    const int r = x * kTileRows + row;
+    const int my_vector = r < rows ? r / p.group : 0;
+    const int my_head = item.kv_head * p.group + (r < rows ? r % p.group : 0);
+    const int4 vec = fits ? p.vectors[item.first_vector + my_vector] : make_int4(0, 0, 0, 0);
+    const int limit = (item.causal != 0 ? min(item.end_token, vec.y + 1) : item.end_token) - item.first_token;
+    const float power = QUANT && count > 0 ? row_power[r] : 1.0f;
+    float m = -INFINITY, l = 0.0f;
+    bool ok = true;
+    for (int j = 0; j < tiles[x]; ++j) {
+      ok = mbar_wait_parked(s_ready + 8 * x, j & 1);
+      if (!ok) {
+        give_up();
+        break;
+      }
+      umma::fence_after_sync();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tile::ld32(s_tmem + 32 * c, s[c]);
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        tile::wait_ld32(s[c]);
+      }
+      if constexpr (QUANT) {
+        // the page's key scale and the row's power of two
+        const float* factors = reinterpret_cast<const float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
+        const int tokens_per_factor = p.page_size;  // 16 or 32
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float f = factors[(c * 32 + h * 16) / tokens_per_factor] * power;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              s[c][h * 16 + i] = __float_as_uint(__uint_as_float(s[c][h * 16 + i]) * f);
+            }
+          }
+        }
+      }
+      if ((j + 1) * kTileTokens > unmasked[x]) {
+        const int seen = limit - j * kTileTokens;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            s[c][i] = c * 32 + i < seen ? s[c][i] : 0xff800000u;
+          }
+        }
+      }
+      float top[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        top[c] = __uint_as_float(s[c][0]);
+#pragma unroll
+        for (int i = 1; i < 32; ++i) {
+          top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+        }
+      }
+      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      if (j == 0) {
+        m = m_new;
+      } else if (__any_sync(0xffffffffu, m_new > m + kLazyGrowth)) {
+        const float alpha = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - m_new);
+        m = m_new;
+        l *= alpha;
+#pragma unroll
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tile::ld32(o_tmem + c, o);
+          tile::wait_ld32(o);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          }
+          st32_tmem(o_tmem + c, o);
+        }
+      }
+      if constexpr (QUANT) {  // the tile's value scales come with its values
+        const int index = 2 * j + 1;
+        ok = mbar_wait_parked(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
+        if (!ok) {
+          give_up();
+          break;
+        }
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float prob[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int column = half * 64 + 2 * i + e;
+            prob[e] = fk_page_decode::exp2_quick(__uint_as_float(s[column / 32][column % 32]) - ref);
+            sum[e] += prob[e];
+          }
+          if constexpr (QUANT) {
+            const float4 f = value_factors[half * 16 + i / 2];
+            prob[0] *= f.x;
+            prob[1] *= f.y;
+            prob[2] *= f.z;
+            prob[3] *= f.w;
+          }
+          packed[i] = pack_bf16(prob[0], prob[1]);
+          packed[i + 1] = pack_bf16(prob[2], prob[3]);
+        }
+        st32_tmem(s_tmem + 32 * half, packed);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      umma::wait_st();
+      umma::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) {
+        umma::mbar_arrive(p_ready + 8 * x);
+      }
+    }
+    // ---- results --------------------------------------------------------------------------------
+    const bool write_row = fits && r < rows && vec.x >= 0 && vec.x < p.num_rows;
+    if (tiles[x] > 0 && ok && !mbar_wait_parked(o_final + 8 * x, 0)) {
+      give_up();
+      ok = false;
+    }
+    if (ok && x * kTileRows < rows && fits) {
+      umma::fence_after_sync();
+      const bool direct = item.partial < 0;
+      const bool slot_fits = direct || (item.partial < vec.w && vec.z >= 0 && vec.z + item.partial < p.num_partials);
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      uint16_t* out = p.output + (static_cast<size_t>(vec.x) * p.num_q_heads + my_head) * D;
+      float* part = p.partials + (static_cast<size_t>(vec.z + item.partial) * p.num_q_heads + my_head) * (D + 4);
+#pragma unroll
+      for (int c = 0; c < D; c += 32) {
+        uint32_t o[32];
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          o[i] = 0u;
+        }
+        if (tiles[x] > 0) {
+          tile::ld32(o_tmem + c, o);
+          tile::wait_ld32(o);
+        }
+        if (write_row && slot_fits) {
+          if (direct) {
+#pragma unroll
+            for (int i = 0; i < 32; i += 8) {
+              uint4 w;
+              w.x = pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+              w.y = pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+              w.z = pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+              w.w = pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+              *reinterpret_cast<uint4*>(out + c + i) = w;
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+            }
+          }
+        }
+      }
+      if (write_row && slot_fits && !direct) {
+        *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+      }
+    }
+  } else {
+    tile::registers_down<L::kOtherRegisters>();
+    if (warp == 8 && lane == 0 && count > 0) {
+      // ---- MMA issuer ---------------------------------------------------------------------------
+      int slot = 0;
+      uint32_t slot_parity = 0;
+      auto next_slot = [&]() {
+        if (++slot == L::kSlots) {
+          slot = 0;
+          slot_parity ^= 1u;
+        }
+      };
+      auto scores = [&](int x, uint32_t k_base) {
+        const uint64_t a = rows_desc(base + L::kQueries + x * L::kOperandBytes);
+        const uint64_t b = rows_desc(k_base);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint64_t step = static_cast<uint64_t>((k / 4) * (L::kHalfBytes >> 4) + (k % 4) * 2);
+          mma_f16_ss(tmem + x * kTileTokens, a + step, b + step, kScoresDesc, k == 0 ? 0u : 1u);
+        }
+        umma::commit(s_ready + 8 * x);
+      };
+      bool ok = mbar_wait_parked(q_ready, 0) && mbar_wait_parked(full, 0);
+      if (ok) {
+        umma::fence_after_sync();
+        for (int x = 0; x < 2; ++x) {
+          if (tiles[x] > 0) {
+            scores(x, base + L::kRing);
+          }
+        }
+        umma::commit(empty);
+        next_slot();
+      }
+      for (int j = 0; ok && j < count; ++j) {
+        const int v_slot = slot;
+        const uint32_t v_base = base + L::kRing + v_slot * L::kOperandBytes;
+        ok = mbar_wait_parked(full + 8 * v_slot, slot_parity);
+        if (ok && !QUANT && clear_needed && j == count - 1) {
+          umma::mbar_arrive(v_landed);
+          ok = mbar_wait_parked(v_clear, 0);
+        }
+        next_slot();
+        const int k_slot = slot;
+        const bool more = j + 1 < count;
+        if (ok && more) {
+          ok = mbar_wait_parked(full + 8 * k_slot, slot_parity);
+        }
+        for (int x = 0; ok && x < 2; ++x) {
+          if (j < tiles[x]) {
+            ok = mbar_wait_parked(p_ready + 8 * x, j & 1);
+            if (!ok) {
+              break;
+            }
+            umma::fence_after_sync();
+            const uint64_t b = columns_desc(v_base);
+#pragma unroll
+            for (int k = 0; k < kTileTokens / 16; ++k) {
+              umma::mma_f16_ts(tmem + 256 + x * D, tmem + x * kTileTokens + 8 * k, b + k * (2048 >> 4), kValuesDesc,
+                               j == 0 && k == 0 ? 0u : 1u);
+            }
+            if (j + 1 == tiles[x]) {
+              umma::commit(o_final + 8 * x);
+            }
+          }
+          if (j + 1 < tiles[x]) {
+            scores(x, base + L::kRing + k_slot * L::kOperandBytes);
+          }
+        }
+        if (ok) {
+          umma::commit(empty + 8 * v_slot);
+          if (more) {
+            umma::commit(empty + 8 * k_slot);
+            next_slot();
+          }
+        }
+      }
+      if (!ok) {
+        give_up();
+      }
+    } else if (warp == 9 && count > 0) {
+      // ---- copies -------------------------------------------------------------------------------
+      // Lane i < pages_per_tile fetches page i of a tile; its ids are read one tile ahead (and, for
+      // 8-bit pages, the keys' scales).
+      const int pages_per_tile = kTileTokens / p.page_size;
+      const int entry = item.entry + item.first_token / p.page_size;
+      const int pages = (loaded + p.page_size - 1) / p.page_size;
+      const uint32_t bars_full = QUANT ? raw_full : full;
+      const uint32_t bars_empty = QUANT ? raw_empty : empty;
+      constexpr int kSlotCount = QUANT ? L::kRawSlots : L::kSlots;
+      auto page_of = [&](int j) -> int {
+        const int i = j * pages_per_tile + lane;
+        if (lane >= pages_per_tile || i >= pages) {
+          return -1;
+        }
+        const int page = __ldg(p.page_ids + entry + i);
+        return min(max(page, 0), p.num_pages - 1);
+      };
+      auto scales_of = [&](int page) -> float2 {
+        float2 v = make_float2(0.0f, 0.0f);
+        if (QUANT && page >= 0) {
+          const float* src = p.key_scales + (static_cast<size_t>(page) * p.num_kv_heads + item.kv_head) * kBlocks;
+          v = kBlocks == 2 ? __ldg(reinterpret_cast<const float2*>(src)) : make_float2(__ldg(src), 0.0f);
+        }
+        return v;
+      };
+      int slot = 0;
+      uint32_t uses = 0;  // how often the ring has gone round
+      int issued = 0;
+      bool ok = true;
+      int page = page_of(0);
+      float2 key_scale = scales_of(page);
+      int next_page = count > 1 ? page_of(1) : -1;
+      for (int j = 0; ok && j < count; ++j) {
+        const float2 next_scale = scales_of(next_page);
+        const int after_page = j + 2 < count ? page_of(j + 2) : -1;
+        const int here = min(pages_per_tile, pages - j * pages_per_tile);  // pages of this tile
+        for (int which = 0; which < 2; ++which) {  // keys, then values
+          if (uses > 0) {
+            ok = mbar_wait_parked(bars_empty + 8 * slot, (uses - 1) & 1);
+            if (!ok) {
+              break;
+            }
+          }
+          const uint32_t bar = bars_full + 8 * slot;
+          if constexpr (QUANT) {
+            const uint32_t page_bytes = p.page_size * D;
+            const uint32_t scale_bytes = which == 1 ? p.page_size * kBlocks * 4 : 0;
+            if (which == 0 && lane < here) {
+              *reinterpret_cast<float2*>(smem + L::kRawKeyScales + slot * 64 + lane * 8) = key_scale;
+            }
+            proxy_fence_async();  // the slot was read through the generic proxy
+            __syncwarp();
+            if (lane == 0) {
+              mbar_expect_tx(bar, here * (page_bytes + scale_bytes));
+            }
+            __syncwarp();
+            if (lane < here) {
+              const size_t page_head = static_cast<size_t>(page) * p.num_kv_heads + item.kv_head;
+              const uint32_t dst = base + L::kRaw + slot * L::kRawSlotBytes;
+              fk_page_decode::bulk_copy_plain(dst + lane * page_bytes,
+                                              (which == 0 ? p.key_pages : p.value_pages) + page_head * page_bytes,
+                                              page_bytes, bar);
+              if (which == 1) {
+                fk_page_decode::bulk_copy_plain(dst + L::kRawBytes + lane * scale_bytes,
+                                                p.value_scales + page_head * (p.page_size * kBlocks), scale_bytes, bar);
+              }
+            }
+          } else {
+            if (lane == 0) {
+              mbar_expect_tx(bar, here * p.page_size * (D * 2));
+            }
+            __syncwarp();
+            if (lane < here) {
+              const int y = (page * p.num_kv_heads + item.kv_head) * p.page_size;
+              const uint32_t dst = base + L::kRing + slot * L::kOperandBytes + lane * p.page_size * 128;
+#pragma unroll
+              for (int h = 0; h < kBlocks; ++h) {
+                tma_load_2d(dst + h * L::kHalfBytes, which == 0 ? &key_map : &value_map, 64 * h, y, bar);
+              }
+            }
+          }
+          ++issued;
+          if (++slot == kSlotCount) {
+            slot = 0;
+            ++uses;
+          }
+        }
+        page = next_page;
+        key_scale = next_scale;
+        next_page = after_page;
+      }
+      if (!ok) {
+        give_up();
+        // let the copies in flight land before the shared memory is handed on
+        for (int i = max(0, issued - kSlotCount); i < issued; ++i) {
+          if (!mbar_wait_parked(bars_full + 8 * (i % kSlotCount), (i / kSlotCount) & 1)) {
+            break;
+          }
+        }
+      }
+    } else if (!QUANT && warp == 10 && clear_needed) {
+      // ---- value rows behind the end ------------------------------------------------------------
+      // The issuer says when they have landed: it follows the ring's phases one by one, and a wait for
+      // a later phase's parity would be over at once.
+      const int slot = (2 * count - 1) % L::kSlots;  // the last tile's values, in the order of the copies
+      if (mbar_wait_parked(v_landed, 0)) {
+        const int valid = loaded - (count - 1) * kTileTokens;
+        const uint32_t v_base = base + L::kRing + slot * L::kOperandBytes;
+        for (int idx = lane; idx < (kTileTokens - valid) * kChunks; idx += 32) {
+          sts128(v_base + operand_chunk(valid + idx / kChunks, idx % kChunks), make_uint4(0u, 0u, 0u, 0u));
+        }
+        proxy_fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          umma::mbar_arrive(v_clear);
+        }
+      } else {
+        give_up();
+      }
+    } else if (QUANT && warp >= 12 && count > 0) {
+      // ---- 8-bit tiles to 16 bits ---------------------------------------------------------------
+      constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
+      constexpr bool kShift = KV == kKvFp8;        // e4m3 keys by bit operations, times 2^-8
+      const int t = tid - 384;
+      const int chunk = t % kChunks;
+      const int block = chunk / 8;
+      int raw_slot = 0, slot = 0;
+      uint32_t raw_uses = 0, uses = 0;
+      bool ok = true;
+      for (int i = 0; ok && i < 2 * count; ++i) {
+        const int j = i >> 1;
+        const bool keys = (i & 1) == 0;
+        ok = mbar_wait_parked(raw_full + 8 * raw_slot, raw_uses & 1) &&
+             (uses == 0 || mbar_wait_parked(empty + 8 * slot, (uses - 1) & 1));
+        if (!ok) {
+          break;
+        }
+        const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
+        const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
+        const int valid = min(kTileTokens, loaded - j * kTileTokens);
+        if (keys) {
+          const float2* scales = reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64);
+          float* factors = reinterpret_cast<float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
+          if (t < kTileTokens / p.page_size) {
+            const float2 s = scales[t];
+            factors[t] = fmaxf(s.x, s.y) * (kShift ? 256.0f : 1.0f);
+          }
+#pragma unroll 4
+          for (int row = t / kChunks; row < valid; row += kRowsPerPass) {
+            const uint2 w = lds64(from + row * D + chunk * 8);
+            uint4 out;
+            fk_page_decode::bytes_to_half2<KV, kShift>(w.x, out.x, out.y);
+            fk_page_decode::bytes_to_half2<KV, kShift>(w.y, out.z, out.w);
+            if constexpr (kBlocks == 2) {
+              const float2 s = scales[row / p.page_size];
+              const float larger = fmaxf(s.x, s.y);
+              const float mine = block == 0 ? s.x : s.y;
+              const __half2 ratio = __float2half2_rn(larger > 0.0f ? mine / larger : 0.0f);
+              __half2* h = reinterpret_cast<__half2*>(&out);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                h[e] = __hmul2(h[e], ratio);
+              }
+            }
+            sts128(to + operand_chunk(row, chunk), out);
+          }
+        } else {
+          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes);
+          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens;
+#pragma unroll 4
+          for (int row = t / kChunks; row < kTileTokens; row += kRowsPerPass) {
+            uint4 out = make_uint4(0u, 0u, 0u, 0u);
+            float larger = 0.0f;
+            if (row < valid) {
+              const uint2 w = lds64(from + row * D + chunk * 8);
+              float a[4], b[4];
+              bytes_to_float4<KV>(w.x, a);
+              bytes_to_float4<KV>(w.y, b);
+              larger = scales[row * kBlocks];
+              if constexpr (kBlocks == 2) {
+                const float2 s = *reinterpret_cast<const float2*>(scales + row * 2);
+                larger = fmaxf(s.x, s.y);
+                const float ratio = larger > 0.0f ? (block == 0 ? s.x : s.y) / larger : 0.0f;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  a[e] *= ratio;
+                  b[e] *= ratio;
+                }
+              }
+              out = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3]));
+            }
+            if (chunk == 0) {
+              factors[row] = larger;
+            }
+            sts128(to + operand_chunk(row, chunk), out);
+          }
+        }
+        proxy_fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          umma::mbar_arrive(full + 8 * slot);
+          umma::mbar_arrive(raw_empty + 8 * raw_slot);
+        }
+        if (++slot == L::kSlots) {
+          slot = 0;
+          ++uses;
+        }
+        if (++raw_slot == L::kRawSlots) {
+          raw_slot = 0;
+          ++raw_uses;
+        }
+      }
+      if (!ok) {
+        give_up();
+      }
+    }
+  }
+
+  __syncwarp();
+  umma::fence_before_sync();
+  __syncthreads();
+  umma::fence_after_sync();
+  if (warp == 8) {
+    if (*fail_flag != 0u) {
+      if (lane == 0) {
+        umma::commit(drain);  // MMAs still in flight, if any
+      }
+      __syncwarp();
+      (void)mbar_wait_parked(drain, 0);
+    }
+    umma::tmem_dealloc(tmem, 512);
+  }
+}
+
+}  // namespace fk_paged_kv
