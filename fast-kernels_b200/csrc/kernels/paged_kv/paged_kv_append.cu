@@ -46,9 +46,18 @@ int fail_cuda(const char* what, cudaError_t err) {
 }
 
 void fill_rope_table(RopeTable* table, int head_dim, float theta) {
-  for (int i = 0; i < head_dim / 2; ++i) {
-    table->turns[i] = std::pow(static_cast<double>(theta), -2.0 * i / head_dim) / 6.283185307179586476925286766559;
+  // 64 powers take longer than the rest of a call; a thread's calls have the same ones nearly always
+  thread_local RopeTable kept;
+  thread_local int kept_dim = 0;
+  thread_local float kept_theta = 0.0f;
+  if (kept_dim != head_dim || kept_theta != theta) {
+    for (int i = 0; i < head_dim / 2; ++i) {
+      kept.turns[i] = std::pow(static_cast<double>(theta), -2.0 * i / head_dim) / 6.283185307179586476925286766559;
+    }
+    kept_dim = head_dim;
+    kept_theta = theta;
   }
+  *table = kept;
 }
 
 }  // namespace fk_paged_kv

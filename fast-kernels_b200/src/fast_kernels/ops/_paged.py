@@ -9,10 +9,18 @@ from typing import Any, Callable
 
 import numpy as np
 
-from fast_kernels.ops.clustered_page_decode import _SCALE_BLOCK, PagedKVCache, _require_layout, _torch
+from fast_kernels.ops.clustered_page_decode import (
+    _SCALE_BLOCK,
+    PagedKVCache,
+    _require_cuda_backend,
+    _require_layout,
+    _torch,
+)
 
 _ROW_ALIGN = 16  # bytes
 _UPLOAD_ALIGN = 128  # int32 words: 512 bytes
+_backend: Any = None
+_HERE = nullcontext()
 
 
 def require_geometry(*, num_kv_heads: int, head_dim: int, page_size: int, kv_layout: str, num_q_heads: int | None = None) -> str:
@@ -80,23 +88,41 @@ def remembered(plans: OrderedDict, made_from: tuple, build: Callable[[], Any], u
     return plan
 
 
-def on_device(kept: dict[int, Any], device: Any, host: dict[str, np.ndarray]) -> dict[str, Any]:
-    """The descriptor tables as int32 tensors on `device`, uploaded once per device in one copy."""
-    torch = _torch()
-    stream = torch.cuda.current_stream(device)
+def backend() -> Any:
+    """The native module; raises where it is missing or was built without CUDA."""
+    global _backend
+    if _backend is None:
+        _backend = _require_cuda_backend()
+    return _backend
+
+
+def current_stream(device: Any) -> int:
+    """Handle of the current stream of `device`."""
+    return _torch()._C._cuda_getCurrentRawStream(device.index)
+
+
+def on_device(kept: dict[int, Any], device: Any, stream: int, host: Callable[[], dict[str, np.ndarray]]) -> dict[str, int]:
+    """Addresses of the descriptor tables as int32 arrays on `device`, for a launch on `stream`; uploaded once per device
+    in one copy."""
     entry = kept.get(device.index)
     if entry is None:
-        parts, sizes = [], []
-        for values in host.values():
+        torch = _torch()
+        tables = host()
+        parts, starts, at = [], {}, 0
+        for name, values in tables.items():
             gap = -values.size % _UPLOAD_ALIGN
             parts += [np.ascontiguousarray(values, dtype=np.int32).reshape(-1), np.zeros(gap, dtype=np.int32)]
-            sizes += [values.size, gap]
+            starts[name] = at
+            at += 4 * (values.size + gap)
         block = torch.from_numpy(np.concatenate(parts)).to(device=device)
-        entry = kept[device.index] = (block, dict(zip(host, block.split(sizes)[::2])), stream.cuda_stream)
-    block, tables, home = entry
-    if stream.cuda_stream != home and not torch.cuda.is_current_stream_capturing():
-        block.record_stream(stream)  # the plan may go away before that stream is done with it
-    return tables
+        base = block.data_ptr()
+        entry = kept[device.index] = (block, {name: base + start for name, start in starts.items()}, stream)
+    block, addresses, home = entry
+    if stream != home:
+        torch = _torch()
+        if not torch.cuda.is_current_stream_capturing():
+            block.record_stream(torch.cuda.current_stream(device))  # the plan may go away before that stream is done with it
+    return addresses
 
 
 def check_rows(tensor: Any, *, name: str, shape: tuple[int, ...], device: Any) -> None:
@@ -106,18 +132,18 @@ def check_rows(tensor: Any, *, name: str, shape: tuple[int, ...], device: Any) -
         raise TypeError(f"{name} must be a torch.Tensor")
     if tensor.ndim != 3:
         raise ValueError(f"{name} must be 3D")
-    if tensor.dtype != torch.bfloat16:
+    if tensor.dtype is not torch.bfloat16:
         raise TypeError(f"{name} must have dtype {torch.bfloat16}")
-    if not tensor.is_cuda:
-        raise ValueError(f"{name} must be a CUDA tensor")
     if tensor.device != device:
+        if not tensor.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor")
         raise ValueError(f"all CUDA tensors must be on the same device: {name}={tensor.device}, key_pages={device}")
-    if tuple(tensor.shape) != shape:
+    if tensor.shape != shape:
         raise ValueError(f"{name} must be shaped {list(shape)}, got {list(tensor.shape)}")
-    if tensor.numel() == 0:
+    if 0 in shape:
         return
-    if tensor.stride(2) != 1 or tensor.data_ptr() % _ROW_ALIGN or any(
-            tensor.stride(d) % 8 for d in (0, 1) if tensor.shape[d] > 1):
+    rows, heads, elements = tensor.stride()
+    if elements != 1 or tensor.data_ptr() % _ROW_ALIGN or (rows % 8 and shape[0] > 1) or (heads % 8 and shape[1] > 1):
         raise ValueError(f"{name} must have contiguous rows that start on 16-byte boundaries")
 
 
@@ -138,47 +164,56 @@ def check_turned_keys(cache: PagedKVCache, rope_theta: float) -> None:
 
 def row_strides(tensor: Any) -> tuple[int, int]:
     """Token and head strides in elements; the stride of a dimension of one entry is never walked."""
-    return tuple(tensor.stride(d) if tensor.shape[d] > 1 else 0 for d in (0, 1))
+    rows, heads, _ = tensor.stride()
+    return rows if tensor.shape[0] > 1 else 0, heads if tensor.shape[1] > 1 else 0
 
 
 def check_cache(cache: PagedKVCache, plan: Any) -> Any:
     """The cache's tensors against its own description and the plan's; returns its device."""
     torch = _torch()
-    for name in ("num_kv_heads", "head_dim", "page_size", "kv_layout"):
-        if getattr(cache, name) != getattr(plan, name):
-            raise ValueError(f"the plan was made for {name}={getattr(plan, name)}, the cache has {getattr(cache, name)}")
+    if (cache.num_kv_heads, cache.head_dim, cache.page_size, cache.kv_layout) != (
+            plan.num_kv_heads, plan.head_dim, plan.page_size, plan.kv_layout):
+        for name in ("num_kv_heads", "head_dim", "page_size", "kv_layout"):
+            if getattr(cache, name) != getattr(plan, name):
+                raise ValueError(f"the plan was made for {name}={getattr(plan, name)}, the cache has {getattr(cache, name)}")
     device = cache.key_pages.device
-    pages = int(cache.key_pages.shape[0])
-    element = {"bf16_kv": torch.bfloat16, "fp8_kv": torch.uint8, "int8_kv": torch.int8}[cache.kv_layout]
+    pages = cache.key_pages.shape[0]
     shape = (pages, cache.num_kv_heads, cache.page_size, cache.head_dim)
-    blocks = cache.head_dim // _SCALE_BLOCK
-    wanted = [("key_pages", cache.key_pages, element, shape), ("value_pages", cache.value_pages, element, shape)]
-    if cache.kv_layout != "bf16_kv":
-        wanted += [("key_scales", cache.key_scales, torch.float32, (*shape[:2], blocks)),
-                   ("value_scales", cache.value_scales, torch.float32, (*shape[:3], blocks))]
-    for name, tensor, dtype, size in wanted:
-        if not isinstance(tensor, torch.Tensor):
-            raise TypeError(f"{name} must be a torch.Tensor")
-        if tensor.dtype != dtype:
-            raise TypeError(f"{name} must have dtype {dtype}")
-        if tuple(tensor.shape) != size:
-            raise ValueError(f"{name} must be shaped {list(size)}, got {list(tensor.shape)}")
-        if not tensor.is_cuda:
-            raise ValueError(f"{name} must be a CUDA tensor")
-        if tensor.device != device:
-            raise ValueError(f"all CUDA tensors must be on the same device: {name}={tensor.device}, key_pages={device}")
-        if not tensor.is_contiguous():
-            raise ValueError(f"{name} must be contiguous")
+    if cache.kv_layout == "bf16_kv":
+        _check_pages("key_pages", cache.key_pages, torch.bfloat16, shape, device)
+        _check_pages("value_pages", cache.value_pages, torch.bfloat16, shape, device)
+    else:
+        element = torch.uint8 if cache.kv_layout == "fp8_kv" else torch.int8
+        blocks = cache.head_dim // _SCALE_BLOCK
+        _check_pages("key_pages", cache.key_pages, element, shape, device)
+        _check_pages("value_pages", cache.value_pages, element, shape, device)
+        _check_pages("key_scales", cache.key_scales, torch.float32, (pages, shape[1], blocks), device)
+        _check_pages("value_scales", cache.value_scales, torch.float32, (*shape[:3], blocks), device)
     if plan.largest_page >= pages:
         raise ValueError(f"the plan names page {plan.largest_page}, the cache has {pages}")
     return device
 
 
+def _check_pages(name: str, tensor: Any, dtype: Any, shape: tuple[int, ...], device: Any) -> None:
+    if not isinstance(tensor, _torch().Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if tensor.dtype is not dtype:
+        raise TypeError(f"{name} must have dtype {dtype}")
+    if tensor.shape != shape:
+        raise ValueError(f"{name} must be shaped {list(shape)}, got {list(tensor.shape)}")
+    if not tensor.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    if tensor.device != device:
+        raise ValueError(f"all CUDA tensors must be on the same device: {name}={tensor.device}, key_pages={device}")
+    if not tensor.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
 def current(device: Any) -> Any:
     """Makes `device` the current one for a launch, where it is not already."""
     torch = _torch()
-    return nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def address(tensor: Any | None) -> int:
-    return 0 if tensor is None else int(tensor.data_ptr())
+    return 0 if tensor is None else tensor.data_ptr()

@@ -35,7 +35,6 @@ from fast_kernels.ops.clustered_page_decode import (
     KvLayout,
     PagedKVCache,
     _layout_id,
-    _require_cuda_backend,
     _torch,
 )
 
@@ -60,8 +59,9 @@ class PagedKVAppendPlan:
     def num_segments(self) -> int:
         return int(self.segments_cpu.shape[0])
 
-    def device_tensors(self, device: Any) -> dict[str, Any]:
-        return _paged.on_device(self._device_cache, device, {"segments": self.segments_cpu.numpy()})
+    def device_tables(self, device: Any, stream: int) -> dict[str, int]:
+        """Addresses of the tables on `device`, for a launch on `stream`; uploaded once per device."""
+        return _paged.on_device(self._device_cache, device, stream, lambda: {"segments": self.segments_cpu.numpy()})
 
 
 def empty_paged_kv(*, num_pages: int, page_table: Any, seq_lens: Any, num_kv_heads: int, head_dim: int, page_size: int,
@@ -145,8 +145,7 @@ def paged_kv_append(
     after the other; views into a fused projection's rows will do) into the cache's pages. Either
     `append_lens` or a `plan` says how many tokens each request gets. Returns the cache with the new
     `seq_lens`; its pages are the same tensors."""
-    torch = _torch()
-    native = _require_cuda_backend()
+    native = _paged.backend()
     if plan is None:
         if append_lens is None:
             raise ValueError("paged_kv_append needs append_lens or a plan")
@@ -163,12 +162,12 @@ def paged_kv_append(
         raise ValueError("rotated key caches must record key_rope_theta")
     if plan.num_tokens:
         with _paged.current(device):
+            stream = _paged.current_stream(device)
             native.paged_kv_append_forward(
-                _paged.address(keys), _paged.address(values), *_paged.row_strides(keys), *_paged.row_strides(values),
-                _paged.address(cache.key_pages), _paged.address(cache.value_pages), _paged.address(cache.key_scales),
-                _paged.address(cache.value_scales), _paged.address(plan.device_tensors(device)["segments"]),
-                plan.num_segments, plan.num_tokens, int(cache.key_pages.shape[0]), plan.num_kv_heads, plan.head_dim,
-                plan.page_size, _layout_id(plan.kv_layout), int(cache.keys_are_rotated),
-                float(cache.key_rope_theta) if cache.keys_are_rotated else 1.0,
-                int(torch.cuda.current_stream(device).cuda_stream))
+                keys.data_ptr(), values.data_ptr(), *_paged.row_strides(keys), *_paged.row_strides(values),
+                cache.key_pages.data_ptr(), cache.value_pages.data_ptr(), _paged.address(cache.key_scales),
+                _paged.address(cache.value_scales), plan.device_tables(device, stream)["segments"], plan.num_segments,
+                plan.num_tokens, cache.key_pages.shape[0], plan.num_kv_heads, plan.head_dim, plan.page_size,
+                _layout_id(plan.kv_layout), int(cache.keys_are_rotated),
+                float(cache.key_rope_theta) if cache.keys_are_rotated else 1.0, stream)
     return dataclasses.replace(cache, seq_lens=plan.seq_lens_after_cpu)

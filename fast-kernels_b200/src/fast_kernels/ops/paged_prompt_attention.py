@@ -24,7 +24,7 @@ from typing import Any
 import numpy as np
 
 from fast_kernels.ops import _paged, _paged_items
-from fast_kernels.ops.clustered_page_decode import KvLayout, PagedKVCache, _layout_id, _require_cuda_backend, _torch
+from fast_kernels.ops.clustered_page_decode import KvLayout, PagedKVCache, _layout_id, _torch
 
 _PLANS: OrderedDict = OrderedDict()
 
@@ -49,8 +49,9 @@ class PagedPromptPlan:
     def num_items(self) -> int:
         return int(self.items_cpu.shape[0])
 
-    def device_tensors(self, device: Any) -> dict[str, Any]:
-        return _paged.on_device(self._device_cache, device, {
+    def device_tables(self, device: Any, stream: int) -> dict[str, int]:
+        """Addresses of the tables on `device`, for a launch on `stream`; uploaded once per device."""
+        return _paged.on_device(self._device_cache, device, stream, lambda: {
             "page_ids": self.page_ids_cpu.numpy(), "vectors": self.vectors_cpu.numpy(), "items": self.items_cpu.numpy()})
 
 
@@ -129,7 +130,7 @@ def paged_prompt_attention(
     a fused projection's rows will do), not yet turned by their positions. Either `query_lens` or a `plan` says how
     many tokens each request has."""
     torch = _torch()
-    native = _require_cuda_backend()
+    native = _paged.backend()
     if not isinstance(query, torch.Tensor):
         raise TypeError("query must be a torch.Tensor")
     if query.ndim != 3:
@@ -151,17 +152,18 @@ def paged_prompt_attention(
     else:
         _paged.check_output(output, shape=shape, device=device)
     if plan.num_tokens:
-        tables = plan.device_tensors(device)
         scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(plan.head_dim)
         with _paged.current(device):
-            partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32,
-                                   device=device) if plan.num_partials else None
+            stream = _paged.current_stream(device)
+            tables = plan.device_tables(device, stream)
+            partials = None
+            if plan.num_partials:
+                partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
             native.paged_attention_forward(
-                _paged.address(query), *_paged.row_strides(query), _paged.address(cache.key_pages),
-                _paged.address(cache.value_pages), _paged.address(cache.key_scales), _paged.address(cache.value_scales),
-                _paged.address(tables["page_ids"]), _paged.address(tables["vectors"]), _paged.address(tables["items"]),
-                _paged.address(output), _paged.address(partials), plan.num_tokens, int(plan.page_ids_cpu.shape[0]),
-                plan.num_tokens, plan.num_items, plan.num_partials, int(cache.key_pages.shape[0]), plan.num_q_heads,
+                query.data_ptr(), *_paged.row_strides(query), cache.key_pages.data_ptr(), cache.value_pages.data_ptr(),
+                _paged.address(cache.key_scales), _paged.address(cache.value_scales), tables["page_ids"], tables["vectors"],
+                tables["items"], output.data_ptr(), _paged.address(partials), plan.num_tokens, plan.page_ids_cpu.shape[0],
+                plan.num_tokens, plan.num_items, plan.num_partials, cache.key_pages.shape[0], plan.num_q_heads,
                 plan.num_kv_heads, plan.head_dim, plan.page_size, _layout_id(plan.kv_layout), float(scale),
-                float(rope_theta), int(torch.cuda.current_stream(device).cuda_stream))
+                float(rope_theta), stream)
     return output

@@ -33,7 +33,6 @@ from fast_kernels.ops.clustered_page_decode import (
     KvLayout,
     PagedKVCache,
     _layout_id,
-    _require_cuda_backend,
     _torch,
     clustered_page_decode,
     plan_clustered_page_decode,
@@ -72,12 +71,12 @@ class SharedPrefixDecodePlan:
     def num_items(self) -> int:
         return int(self.items_cpu.shape[0])
 
-    def device_tensors(self, device: Any) -> dict[str, Any]:
-        tail = self.tail_plan
-        return _paged.on_device(self._device_cache, device, {
+    def device_tables(self, device: Any, stream: int) -> dict[str, int]:
+        """Addresses of the tables on `device`, for a launch on `stream`; uploaded once per device."""
+        return _paged.on_device(self._device_cache, device, stream, lambda: {
             "page_ids": self.page_ids_cpu.numpy(), "vectors": self.vectors_cpu.numpy(), "items": self.items_cpu.numpy(),
             "of_request": self.of_request_cpu.numpy(),
-            **{name: getattr(tail, f"{name}_cpu").numpy() for name in (
+            **{name: getattr(self.tail_plan, f"{name}_cpu").numpy() for name in (
                 "run_base_pages", "run_page_counts", "run_logical_starts", "run_last_page_lens", "request_run_offsets", "seq_lens")}})
 
 
@@ -222,7 +221,7 @@ def shared_prefix_decode(
     """`query` is bf16 [batch, q_heads, head_dim], contiguous, not yet turned by its positions; request b's token is the
     last of its `seq_lens[b]`. The cache's keys are turned ahead of time (`key_rope_theta`)."""
     torch = _torch()
-    native = _require_cuda_backend()
+    native = _paged.backend()
     if not isinstance(query, torch.Tensor):
         raise TypeError("query must be a torch.Tensor")
     if query.ndim != 3:
@@ -244,17 +243,16 @@ def shared_prefix_decode(
         if not plan.runs:
             return clustered_page_decode(query, cache, plan=plan.tail_plan, output=output, softmax_scale=scale,
                                          rope_theta=rope_theta)
-        tables = plan.device_tensors(device)
+        stream = _paged.current_stream(device)
+        tables = plan.device_tables(device, stream)
         partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
+        tail = plan.tail_plan
         native.shared_prefix_decode_forward(
-            _paged.address(query), _paged.address(cache.key_pages), _paged.address(cache.value_pages),
-            _paged.address(cache.key_scales), _paged.address(cache.value_scales), _paged.address(tables["page_ids"]),
-            _paged.address(tables["vectors"]), _paged.address(tables["items"]), _paged.address(tables["of_request"]),
-            _paged.address(tables["run_base_pages"]), _paged.address(tables["run_page_counts"]),
-            _paged.address(tables["run_logical_starts"]), _paged.address(tables["run_last_page_lens"]),
-            _paged.address(tables["request_run_offsets"]), _paged.address(tables["seq_lens"]), _paged.address(output),
-            _paged.address(partials), plan.batch, int(plan.page_ids_cpu.shape[0]), plan.num_items, plan.num_partials,
-            plan.tail_plan.num_runs, plan.tail_plan.max_pages, int(cache.key_pages.shape[0]), plan.num_q_heads,
-            plan.num_kv_heads, plan.head_dim, plan.page_size, _layout_id(plan.kv_layout), float(scale), float(rope_theta),
-            int(torch.cuda.current_stream(device).cuda_stream))
+            query.data_ptr(), cache.key_pages.data_ptr(), cache.value_pages.data_ptr(), _paged.address(cache.key_scales),
+            _paged.address(cache.value_scales), tables["page_ids"], tables["vectors"], tables["items"], tables["of_request"],
+            tables["run_base_pages"], tables["run_page_counts"], tables["run_logical_starts"], tables["run_last_page_lens"],
+            tables["request_run_offsets"], tables["seq_lens"], output.data_ptr(), partials.data_ptr(), plan.batch,
+            plan.page_ids_cpu.shape[0], plan.num_items, plan.num_partials, tail.num_runs, tail.max_pages,
+            cache.key_pages.shape[0], plan.num_q_heads, plan.num_kv_heads, plan.head_dim, plan.page_size,
+            _layout_id(plan.kv_layout), float(scale), float(rope_theta), stream)
     return output

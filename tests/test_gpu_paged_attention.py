@@ -242,7 +242,7 @@ def test_prompts_same_bits_every_time_on_streams_and_in_graphs() -> None:
     plan = ops.plan_paged_prompt_attention(page_table=cache.page_table, seq_lens=cache.seq_lens, query_lens=torch.tensor([40, 100]),
                                            num_q_heads=8, num_kv_heads=2, head_dim=128, page_size=16, kv_layout="fp8_kv", use_cache=False)
     assert plan.num_partials > 0
-    plan.device_tensors(query.device)
+    plan.device_tables(query.device, torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     outputs = []
     for stream in [torch.cuda.Stream() for _ in range(4)]:

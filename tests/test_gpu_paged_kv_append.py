@@ -179,7 +179,7 @@ def test_two_streams_and_a_captured_step() -> None:
     plan = ops.plan_paged_kv_append(page_table=caches[0].page_table, seq_lens=caches[0].seq_lens, append_lens=torch.tensor(new),
                                     num_kv_heads=2, head_dim=128, page_size=16, kv_layout="int8_kv", use_cache=False)
     before, want = _copy(caches[0]), append64(caches[0], keys, values, new)
-    plan.device_tensors(keys.device)
+    plan.device_tables(keys.device, torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     streams = [torch.cuda.Stream() for _ in range(2)]
     for stream, cache in zip(streams, caches):
