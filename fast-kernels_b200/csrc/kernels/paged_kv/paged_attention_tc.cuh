@@ -135,21 +135,43 @@ __device__ __forceinline__ void st32_tmem(uint32_t taddr, const uint32_t (&r)[32
       : "memory");
 }
 
-// Four 8-bit numbers as floats, exactly (e4m3: times 2^-8 where SHIFTED words were asked for).
-template <int KV>
-__device__ __forceinline__ void bytes_to_float4(uint32_t w, float (&x)[4]) {
-  if constexpr (KV == kKvInt8) {
-    const uint32_t u = w ^ 0x80808080u;  // byte + 128 dropped into the mantissa of 2^23
+using fk_page_decode::f32x2;
+using fk_page_decode::fma2;
+using fk_page_decode::mul2;
+using fk_page_decode::pack2;
+using fk_page_decode::unpack2;
+__device__ __forceinline__ f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ f32x2 pair_of(const uint32_t* r) { return pack2(__uint_as_float(r[0]), __uint_as_float(r[1])); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Largest of N values, as two chains.
+template <int N>
+__device__ __forceinline__ float largest_of(const uint32_t* r) {
+  float a = __uint_as_float(r[0]), b = __uint_as_float(r[1]);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      x[i] = __uint_as_float(__byte_perm(u, 0x4B000000u, 0x7540u + i)) - 8388736.0f;
-    }
-  } else {
-    uint32_t a, b;
-    fk_page_decode::bytes_to_half2<fk_page_decode::kKvFp8, false>(w, a, b);
-    const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&a));
-    const float2 hi = __half22float2(*reinterpret_cast<const __half2*>(&b));
-    x[0] = lo.x, x[1] = lo.y, x[2] = hi.x, x[3] = hi.y;
+  for (int i = 2; i + 3 < N; i += 4) {
+    a = max3(a, __uint_as_float(r[i]), __uint_as_float(r[i + 1]));
+    b = max3(b, __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+  }
+  return max3(a, b, max3(a, __uint_as_float(r[N - 2]), __uint_as_float(r[N - 1])));
+}
+
+// Eight fp16 numbers times unit * mine / larger (exactly `unit` for the block that has the larger scale).
+// `unit` undoes the 2^-8 of shifted e4m3 numbers: what is left of the other block must stay clear of
+// fp16's subnormal numbers as far as it can.
+__device__ __forceinline__ void scale_half8(uint4& v, float mine, float larger, float unit) {
+  const __half2 ratio = __float2half2_rn(larger > 0.0f ? unit * __fdividef(mine, larger) : 0.0f);
+  __half2* h = reinterpret_cast<__half2*>(&v);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    h[e] = __hmul2(h[e], ratio);
   }
 }
 
@@ -162,7 +184,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   constexpr int kBlocks = D / 64;          // scale blocks, and halves of an operand
   constexpr int kChunks = D / 8;           // 16-byte chunks of a row
   constexpr uint32_t kScoresDesc = instruction_desc(!QUANT, kTileTokens, false);
-  constexpr uint32_t kValuesDesc = instruction_desc(true, D, true);
+  constexpr uint32_t kValuesDesc = instruction_desc(!QUANT, D, true);
   extern __shared__ __align__(16) uint8_t raw_smem[];
 
   const int tid = static_cast<int>(threadIdx.x);
@@ -349,6 +371,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     const int limit = (item.causal != 0 ? min(item.end_token, vec.y + 1) : item.end_token) - item.first_token;
     const float power = QUANT && count > 0 ? row_power[r] : 1.0f;
     float m = -INFINITY, l = 0.0f;
+    int o_bits = fk_page_decode::kMinExponentBits;  // QUANT: exponent bits of the power of two that O is divided by
     bool ok = true;
     for (int j = 0; j < tiles[x]; ++j) {
       ok = mbar_wait_parked(s_ready + 8 * x, j & 1);
@@ -357,57 +380,62 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         break;
       }
       umma::fence_after_sync();
-      uint32_t s[4][32];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tile::ld32(s_tmem + 32 * c, s[c]);
-      }
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        tile::wait_ld32(s[c]);
-      }
-      if constexpr (QUANT) {
-        // the page's key scale and the row's power of two
-        const float* factors = reinterpret_cast<const float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
-        const int tokens_per_factor = p.page_size;  // 16 or 32
+      uint32_t s[128];
+      {
+        uint32_t(&s4)[4][32] = *reinterpret_cast<uint32_t(*)[4][32]>(s);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
+          tile::ld32(s_tmem + 32 * c, s4[c]);
+        }
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float f = factors[(c * 32 + h * 16) / tokens_per_factor] * power;
+        for (int c = 0; c < 4; ++c) {
+          tile::wait_ld32(s4[c]);
+        }
+      }
+      // QUANT: what 16 neighbouring logits are multiplied by, the page's key scale and the row's power of two
+      float factor[8];
+      if constexpr (QUANT) {
+        const float* factors = reinterpret_cast<const float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              s[c][h * 16 + i] = __float_as_uint(__uint_as_float(s[c][h * 16 + i]) * f);
-            }
-          }
+        for (int g = 0; g < 8; ++g) {
+          factor[g] = factors[p.page_size == 16 ? g : g >> 1] * power;
         }
       }
       if ((j + 1) * kTileTokens > unmasked[x]) {
         const int seen = limit - j * kTileTokens;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int i = 0; i < 128; ++i) {
+          const float logit = QUANT ? __uint_as_float(s[i]) * factor[i / 16] : __uint_as_float(s[i]);
+          s[i] = i < seen ? __float_as_uint(logit) : 0xff800000u;
+        }
+        if constexpr (QUANT) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[c][i] = c * 32 + i < seen ? s[c][i] : 0xff800000u;
+          for (int g = 0; g < 8; ++g) {
+            factor[g] = 1.0f;
           }
         }
       }
       float top[4];
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        top[c] = __uint_as_float(s[c][0]);
-#pragma unroll
-        for (int i = 1; i < 32; ++i) {
-          top[c] = fmaxf(top[c], __uint_as_float(s[c][i]));
+        if constexpr (QUANT) {  // (scales are positive)
+          top[c] = fmaxf(largest_of<16>(s + 32 * c) * factor[2 * c], largest_of<16>(s + 32 * c + 16) * factor[2 * c + 1]);
+        } else {
+          top[c] = largest_of<32>(s + 32 * c);
         }
       }
-      const float m_new = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+      const float m_new = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
+      float carry = 1.0f;  // what O is multiplied by
+      bool rescale = false;
       if (j == 0) {
         m = m_new;
       } else if (__any_sync(0xffffffffu, m_new > m + kLazyGrowth)) {
-        const float alpha = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - m_new);
+        carry = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - m_new);
         m = m_new;
-        l *= alpha;
+        l *= carry;
+        rescale = true;
+      }
+      auto rescale_values = [&]() {
 #pragma unroll
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -415,47 +443,92 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           tile::wait_ld32(o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+            o[i] = __float_as_uint(__uint_as_float(o[i]) * carry);
           }
           st32_tmem(o_tmem + c, o);
         }
-      }
-      if constexpr (QUANT) {  // the tile's value scales come with its values
-        const int index = 2 * j + 1;
+      };
+      const float ref = m == -INFINITY ? 0.0f : m;
+      const f32x2 minus_ref = pack2(-ref, -ref);
+      f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+      if constexpr (!QUANT) {
+        if (rescale) {
+          rescale_values();
+        }
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float a, b;
+            unpack2(add2(pair_of(s + half * 64 + 2 * i), minus_ref), a, b);
+            a = fk_page_decode::exp2_quick(a);
+            b = fk_page_decode::exp2_quick(b);
+            sum[i & 1] = add2(sum[i & 1], pack2(a, b));
+            packed[i] = pack_bf16(a, b);
+          }
+          st32_tmem(s_tmem + 32 * half, packed);
+        }
+      } else {
+        // Weights are the probabilities times their token's value scale, brought to fp16's range by a
+        // power of two of the row's own, kept as lazily as the maximum.
+        const int index = 2 * j + 1;  // the scales come with the tile's values
         ok = mbar_wait_parked(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
         if (!ok) {
           give_up();
           break;
         }
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
+        const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t packed[32];
+        for (int i = 0; i < 128; i += 4) {
+          const f32x2 f = pack2(factor[i / 16], factor[i / 16]);
+          const float4 v = value_factors[i / 4];
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          float prob[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int column = half * 64 + 2 * i + e;
-            prob[e] = fk_page_decode::exp2_quick(__uint_as_float(s[column / 32][column % 32]) - ref);
-            sum[e] += prob[e];
+          for (int e = 0; e < 4; e += 2) {
+            float a, b;
+            unpack2(fma2(pair_of(s + i + e), f, minus_ref), a, b);
+            a = fk_page_decode::exp2_quick(a);
+            b = fk_page_decode::exp2_quick(b);
+            const f32x2 prob = pack2(a, b);
+            sum[e / 2] = add2(sum[e / 2], prob);
+            unpack2(mul2(prob, e == 0 ? pack2(v.x, v.y) : pack2(v.z, v.w)), a, b);
+            s[i + e] = __float_as_uint(a);
+            s[i + e + 1] = __float_as_uint(b);
           }
-          if constexpr (QUANT) {
-            const float4 f = value_factors[half * 16 + i / 2];
-            prob[0] *= f.x;
-            prob[1] *= f.y;
-            prob[2] *= f.z;
-            prob[3] *= f.w;
-          }
-          packed[i] = pack_bf16(prob[0], prob[1]);
-          packed[i + 1] = pack_bf16(prob[2], prob[3]);
         }
-        st32_tmem(s_tmem + 32 * half, packed);
+        const float heaviest = fmaxf(fmaxf(largest_of<32>(s), largest_of<32>(s + 32)), fmaxf(largest_of<32>(s + 64), largest_of<32>(s + 96)));
+        const int bits = fk_page_decode::exponent_bits(heaviest);
+        if (j == 0) {
+          o_bits = bits;
+        } else if (rescale || __any_sync(0xffffffffu, bits > o_bits + (static_cast<int>(kLazyGrowth) << 23))) {
+          // the power follows what the old sum is worth under the new maximum, up or down
+          const float worth = __int_as_float(o_bits) * carry;
+          o_bits = max(bits, fk_page_decode::exponent_bits(worth));
+          carry = worth * fk_page_decode::inverse_power(o_bits);
+          rescale = true;
+        }
+        if (rescale) {
+          rescale_values();
+        }
+        const float shrink = fk_page_decode::inverse_power(o_bits);
+        const f32x2 shrink2 = pack2(shrink, shrink);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t packed[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float a, b;
+            unpack2(mul2(pair_of(s + half * 64 + 2 * i), shrink2), a, b);
+            packed[i] = pack_half(a, b);
+          }
+          st32_tmem(s_tmem + 32 * half, packed);
+        }
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      {
+        float a, b;
+        unpack2(add2(sum[0], sum[1]), a, b);
+        l += a + b;
+      }
       umma::wait_st();
       umma::fence_before_sync();
       __syncwarp();
@@ -463,6 +536,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         umma::mbar_arrive(p_ready + 8 * x);
       }
     }
+    const float values_power = QUANT ? __int_as_float(o_bits) * (KV == kKvFp8 && kBlocks == 1 ? 256.0f : 1.0f) : 1.0f;
     // ---- results --------------------------------------------------------------------------------
     const bool write_row = fits && r < rows && vec.x >= 0 && vec.x < p.num_rows;
     if (tiles[x] > 0 && ok && !mbar_wait_parked(o_final + 8 * x, 0)) {
@@ -473,7 +547,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       umma::fence_after_sync();
       const bool direct = item.partial < 0;
       const bool slot_fits = direct || (item.partial < vec.w && vec.z >= 0 && vec.z + item.partial < p.num_partials);
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      const float inv = l == 0.0f ? 0.0f : values_power / l;
       uint16_t* out = p.output + (static_cast<size_t>(vec.x) * p.num_q_heads + my_head) * D;
       float* part = p.partials + (static_cast<size_t>(vec.z + item.partial) * p.num_q_heads + my_head) * (D + 4);
 #pragma unroll
@@ -501,7 +575,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+              *reinterpret_cast<float4*>(part + c + i) =
+                  make_float4(__uint_as_float(o[i]) * values_power, __uint_as_float(o[i + 1]) * values_power,
+                              __uint_as_float(o[i + 2]) * values_power, __uint_as_float(o[i + 3]) * values_power);
             }
           }
         }
@@ -712,7 +788,8 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     } else if (QUANT && warp >= 12 && count > 0) {
       // ---- 8-bit tiles to 16 bits ---------------------------------------------------------------
       constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
-      constexpr bool kShift = KV == kKvFp8;        // e4m3 keys by bit operations, times 2^-8
+      constexpr bool kShift = KV == kKvFp8;        // e4m3 numbers by bit operations, times 2^-8
+      constexpr float kUnit = kShift ? 256.0f : 1.0f;
       const int t = tid - 384;
       const int chunk = t % kChunks;
       const int block = chunk / 8;
@@ -735,7 +812,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           float* factors = reinterpret_cast<float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
           if (t < kTileTokens / p.page_size) {
             const float2 s = scales[t];
-            factors[t] = fmaxf(s.x, s.y) * (kShift ? 256.0f : 1.0f);
+            factors[t] = fmaxf(s.x, s.y) * (kBlocks == 1 ? kUnit : 1.0f);
           }
 #pragma unroll 4
           for (int row = t / kChunks; row < valid; row += kRowsPerPass) {
@@ -745,14 +822,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
             fk_page_decode::bytes_to_half2<KV, kShift>(w.y, out.z, out.w);
             if constexpr (kBlocks == 2) {
               const float2 s = scales[row / p.page_size];
-              const float larger = fmaxf(s.x, s.y);
-              const float mine = block == 0 ? s.x : s.y;
-              const __half2 ratio = __float2half2_rn(larger > 0.0f ? mine / larger : 0.0f);
-              __half2* h = reinterpret_cast<__half2*>(&out);
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                h[e] = __hmul2(h[e], ratio);
-              }
+              scale_half8(out, block == 0 ? s.x : s.y, fmaxf(s.x, s.y), kUnit);
             }
             sts128(to + operand_chunk(row, chunk), out);
           }
@@ -765,21 +835,14 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
             float larger = 0.0f;
             if (row < valid) {
               const uint2 w = lds64(from + row * D + chunk * 8);
-              float a[4], b[4];
-              bytes_to_float4<KV>(w.x, a);
-              bytes_to_float4<KV>(w.y, b);
+              fk_page_decode::bytes_to_half2<KV, kShift>(w.x, out.x, out.y);
+              fk_page_decode::bytes_to_half2<KV, kShift>(w.y, out.z, out.w);
               larger = scales[row * kBlocks];
               if constexpr (kBlocks == 2) {
                 const float2 s = *reinterpret_cast<const float2*>(scales + row * 2);
                 larger = fmaxf(s.x, s.y);
-                const float ratio = larger > 0.0f ? (block == 0 ? s.x : s.y) / larger : 0.0f;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  a[e] *= ratio;
-                  b[e] *= ratio;
-                }
+                scale_half8(out, block == 0 ? s.x : s.y, larger, kUnit);
               }
-              out = make_uint4(pack_bf16(a[0], a[1]), pack_bf16(a[2], a[3]), pack_bf16(b[0], b[1]), pack_bf16(b[2], b[3]));
             }
             if (chunk == 0) {
               factors[row] = larger;

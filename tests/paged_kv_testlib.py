@@ -172,5 +172,49 @@ def attention64(cache: Any, query: torch.Tensor, rows: list[tuple[int, int]], sc
     return out
 
 
+def attention_terms64(cache: Any, query: torch.Tensor, rows: list[tuple[int, int]], scale: float, theta: float) -> dict[str, torch.Tensor]:
+    """`attention64`, and what its rounding errors are bounded by, per row and query head (and dimension):
+    a = sum_t p_t |v_t|; logit = max_t |scale| sum_i |q_i k_i|; query = sum_i |q_i|; with s_t the larger of a token's value
+    scales (8-bit pages): weight = max_t p_t s_t, weights = sum_t p_t s_t, numbers = sum_t |v_t| / s_t; and the largest key
+    scale of the tokens."""
+    keys, values = cache_values(cache)
+    ps, heads = cache.page_size, cache.num_kv_heads
+    q = rotate64(query.cpu(), [max(0, p) for _, p in rows], theta)
+    group, dim = q.shape[1] // heads, q.shape[2]
+    quantised = cache.kv_layout != "bf16_kv"
+    terms = {name: torch.zeros_like(q) for name in ("out", "a", "numbers")}
+    terms |= {name: torch.zeros((*q.shape[:2], 1), dtype=torch.float64) for name in ("logit", "query", "weight", "weights", "key_scale")}
+    gathered: dict[int, list[torch.Tensor]] = {}
+    for i, (request, position) in enumerate(rows):
+        if position < 0:
+            continue
+        if request not in gathered:
+            most = max(p for r, p in rows if r == request) + 1
+            pages = cache.page_table[request, : -(-most // ps)].long()
+            flat = lambda x: x[pages].permute(1, 0, 2, 3).reshape(heads, -1, x.shape[-1])  # noqa: E731
+            gathered[request] = [flat(keys), flat(values)]
+            if quantised:
+                gathered[request].append(flat(cache.value_scales.cpu().double()).amax(dim=-1, keepdim=True))
+                page_scales = cache.key_scales.cpu().double().amax(dim=-1)[:, :, None, None].expand(-1, -1, ps, -1)
+                gathered[request].append(flat(page_scales))
+        k, v, *scales = (x[:, : position + 1] for x in gathered[request])
+        mine = q[i].reshape(heads, group, dim)
+        p = torch.softmax(torch.einsum("hgd,htd->hgt", mine, k) * scale, dim=-1)
+
+        def put(name: str, x: torch.Tensor) -> None:
+            terms[name][i] = x.reshape(heads * group, -1)
+
+        put("out", torch.einsum("hgt,htd->hgd", p, v))
+        put("a", torch.einsum("hgt,htd->hgd", p, v.abs()))
+        put("logit", abs(scale) * torch.einsum("hgd,htd->hgt", mine.abs(), k.abs()).amax(dim=-1))
+        put("query", mine.abs().sum(dim=-1))
+        if quantised:
+            put("weight", (p * scales[0].transpose(1, 2)).amax(dim=-1))
+            put("weights", (p * scales[0].transpose(1, 2)).sum(dim=-1))
+            put("numbers", (v.abs() / scales[0]).sum(dim=1)[:, None].expand(-1, group, -1))
+            put("key_scale", scales[1].amax(dim=(1, 2))[:, None].expand(-1, group))
+    return terms
+
+
 def default_scale(dim: int) -> float:
     return 1.0 / math.sqrt(dim)

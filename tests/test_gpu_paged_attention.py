@@ -1,12 +1,18 @@
 """paged_prompt_attention and shared_prefix_decode on the GPU against attention in 64 bits over the same bytes.
 
-Tolerances, with u = 2^-8 (half a step of bf16) and h the rounding of the turned query (u for bf16 pages, 2^-11 for 8-bit
-ones). Let a = sum_t p_t |v_t| with the exact weights p.
- * the row is rounded once: u |y|;
- * weights are rounded to bf16 before they meet the values, 8-bit values times their relative scale too: (u, or 2 u) a;
- * a logit is off by at most d = h * scale * sum_i |q_i k_i| (and fp32 sums, well below), which changes every weight by a
-   factor within e^(+-2 d): 2 d a to first order; d is taken at the largest sum over the row's tokens, times 1.1 for the
-   higher orders.
+Tolerances, with u = 2^-8 (half a step of bf16) and h = 2^-11 (half a step of fp16; 2^-25 below 2^-14). Let a = sum_t p_t |v_t|
+with the exact weights p. The row is rounded once: u |y|. The rest, to first order:
+
+bf16 pages: the turned query is rounded to bf16, so that a logit is off by at most d = u * scale * sum_i |q_i k_i| and every
+weight by a factor within e^(+-2 d); weights are rounded to bf16: (u + 2 d) a.
+
+8-bit pages: query, keys and values are fp16. The query and the keys' elements are off by h, the elements of the block that has
+not the page's larger scale by 2 h more (the ratio of the scales, the product), or by 2^-25 of that scale:
+d = scale * (3 h sum_i |q_i k_i| + 2^-25 s_k sum_i |q_i|), one h where there is one block. The same of values and weights:
+(3 h + 2 d) a + 2^-25 sum_t p_t s_t, and, since a weight p_t s_t below 2^-14 of the row's largest W is off by up to 2^-25 W
+however small it is itself, 2^-25 W sum_t |v_t| / s_t.
+
+d is taken at the largest sum over the row's tokens, times 1.1 for the higher orders; fp32 sums are well below all of these.
 The tail of a shared decode rounds less. On top, an element-wise bound that wide says little about a token too many or too
 few in a long row; the counting tests do: keys of zero make all weights equal, and each output counts the tokens of one
 residue, so that one token more or less is seen at once."""
@@ -21,12 +27,11 @@ import pytest
 import torch
 from fast_kernels.native import native_module
 from paged_kv_testlib import (
-    attention64,
-    cache_values,
+    BLOCK,
+    attention_terms64,
     default_scale,
     fragmented_table,
     random_cache,
-    rotate64,
 )
 
 pytestmark = pytest.mark.gpu
@@ -34,6 +39,7 @@ ops = importlib.import_module("fast_kernels.ops")
 LAYOUTS = ("bf16_kv", "fp8_kv", "int8_kv")
 THETA = 10000.0
 U = 2.0**-8
+H = 2.0**-11
 
 
 def _status_ok() -> None:
@@ -46,25 +52,15 @@ def _query(rows: int, heads: int, dim: int, seed: int) -> torch.Tensor:
 
 
 def _assert_rows(got: torch.Tensor, cache, query, rows, scale: float) -> None:
-    want = attention64(cache, query, rows, scale, THETA)
-    magnitudes = dataclasses.replace(cache, value_pages=cache.value_pages.abs() if cache.kv_layout != "fp8_kv" else cache.value_pages & 0x7F)
-    a = attention64(magnitudes, query, rows, scale, THETA)
-    keys, _ = cache_values(cache)
-    turned = rotate64(query.cpu(), [max(0, p) for _, p in rows], THETA).abs()
-    group = turned.shape[1] // cache.num_kv_heads
-    largest = torch.zeros(turned.shape[:2], dtype=torch.float64)
-    gathered = {}
-    for i, (request, position) in enumerate(rows):
-        if position >= 0:
-            if request not in gathered:
-                most = max(p for r, p in rows if r == request) + 1
-                pages = cache.page_table[request, : -(-most // cache.page_size)].long()
-                gathered[request] = keys[pages].abs().permute(1, 0, 2, 3).reshape(cache.num_kv_heads, -1, keys.shape[-1])
-            k = gathered[request][:, : position + 1]
-            largest[i] = torch.einsum("hgd,htd->hgt", turned[i].reshape(cache.num_kv_heads, group, -1), k).amax(dim=-1).flatten()
-    h = U if cache.kv_layout == "bf16_kv" else 2.0**-11
-    d = 1.1 * h * abs(scale) * largest[..., None]
-    bound = U * want.abs() + (U * (1 if cache.kv_layout == "bf16_kv" else 2) + 2 * d) * a + 1e-30
+    terms = attention_terms64(cache, query, rows, scale, THETA)
+    want, a = terms["out"], terms["a"]
+    if cache.kv_layout == "bf16_kv":
+        d = 1.1 * U * terms["logit"]
+        bound = U * want.abs() + (U + 2 * d) * a + 1e-30
+    else:
+        h = H * (3 if cache.head_dim > BLOCK else 1)
+        d = 1.1 * (h * terms["logit"] + 2.0**-25 * abs(scale) * terms["key_scale"] * terms["query"])
+        bound = U * want.abs() + (h + 2 * d) * a + 2.0**-25 * (terms["weights"] + terms["weight"] * terms["numbers"]) + 1e-30
     off = (got.double().cpu() - want).abs()
     assert bool(torch.isfinite(got).all())
     worst = float((off / bound).max()) if off.numel() else 0.0
