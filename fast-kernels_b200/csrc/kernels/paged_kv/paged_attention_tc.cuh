@@ -10,6 +10,10 @@
 // While the softmax warps of one row tile work, the tensor core multiplies for the other. The softmax
 // scale times log2(e) rides on the query, so the exponential is one ex2.
 //
+// The logits are read from tensor memory twice, 32 columns at a time: once for the row's maximum, once
+// for the probabilities. A row of 128 kept in registers in between left the compiler too few of them to
+// overlap one exponential with the next.
+//
 // The running maximum is kept lazily: O is multiplied by 2^(old - new) only when a row's maximum has
 // grown by more than 2^8 since the last time, else P may be up to 2^8 and nothing is lost (bf16 and
 // fp32 have the range). The tensor core is done with O whenever a tile's logits are: their commit
@@ -73,8 +77,8 @@ struct TcLayout {
   static constexpr int kRing = kQueries + 2 * kOperandBytes;
   static constexpr int kRaw = kRing + kSlots * kOperandBytes;
   static constexpr int kKeyFactors = kRaw + kRawSlots * kRawSlotBytes;              // [ring][8 pages]
-  static constexpr int kValueFactors = kKeyFactors + (kQuant ? kFactorRing * 32 : 0);  // [ring][128 tokens]
-  static constexpr int kRawKeyScales = kValueFactors + (kQuant ? kFactorRing * 512 : 0);  // [raw slot][8 pages][2]
+  static constexpr int kValueFactors = kKeyFactors + (kQuant ? kFactorRing * 32 : 0);  // [ring][128 tokens], then their log2
+  static constexpr int kRawKeyScales = kValueFactors + (kQuant ? kFactorRing * 1024 : 0);  // [raw slot][8 pages][2]
   static constexpr int kRowPower = kRawKeyScales + kRawSlots * 64;                  // [256]
   static constexpr int kBarriers = kRowPower + (kQuant ? 1024 : 0);
   static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
@@ -195,7 +199,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   const uint32_t bars = base + L::kBarriers;
   const uint32_t q_ready = bars + 16;
   const uint32_t s_ready = bars + 24;             // [2] logits of a tile are there
-  const uint32_t p_ready = bars + 40;             // [2] probabilities are stored (and O is rescaled)
+  // [half][2] probabilities of a half tile are stored (and O is rescaled). A barrier each: with one for
+  // both, a late issuer would find its phase overtaken by the next.
+  const uint32_t p_ready = bars + 352;
   const uint32_t o_final = bars + 56;             // [2] the last product is done
   const uint32_t v_clear = bars + 72;
   const uint32_t drain = bars + 80;
@@ -213,6 +219,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_ready + 8 * x, 1);
       mbar_init(p_ready + 8 * x, 4);
+      mbar_init(p_ready + 16 + 8 * x, 4);
       mbar_init(o_final + 8 * x, 1);
     }
     mbar_init(v_landed, 1);
@@ -380,124 +387,84 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         break;
       }
       umma::fence_after_sync();
-      uint32_t s[128];
-      {
-        uint32_t(&s4)[4][32] = *reinterpret_cast<uint32_t(*)[4][32]>(s);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tile::ld32(s_tmem + 32 * c, s4[c]);
-        }
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          tile::wait_ld32(s4[c]);
-        }
-      }
       // QUANT: what 16 neighbouring logits are multiplied by, the page's key scale and the row's power of two
       float factor[8];
+      const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
+      const float4* value_logs = value_factors + kFactorRing * 32;
       if constexpr (QUANT) {
         const float* factors = reinterpret_cast<const float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
           factor[g] = factors[p.page_size == 16 ? g : g >> 1] * power;
         }
-      }
-      if ((j + 1) * kTileTokens > unmasked[x]) {
-        const int seen = limit - j * kTileTokens;
-#pragma unroll
-        for (int i = 0; i < 128; ++i) {
-          const float logit = QUANT ? __uint_as_float(s[i]) * factor[i / 16] : __uint_as_float(s[i]);
-          s[i] = i < seen ? __float_as_uint(logit) : 0xff800000u;
-        }
-        if constexpr (QUANT) {
-#pragma unroll
-          for (int g = 0; g < 8; ++g) {
-            factor[g] = 1.0f;
-          }
-        }
-      }
-      float top[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        if constexpr (QUANT) {  // (scales are positive)
-          top[c] = fmaxf(largest_of<16>(s + 32 * c) * factor[2 * c], largest_of<16>(s + 32 * c + 16) * factor[2 * c + 1]);
-        } else {
-          top[c] = largest_of<32>(s + 32 * c);
-        }
-      }
-      const float m_new = fmaxf(fmaxf(m, fmaxf(top[0], top[1])), fmaxf(top[2], top[3]));
-      float carry = 1.0f;  // what O is multiplied by
-      bool rescale = false;
-      if (j == 0) {
-        m = m_new;
-      } else if (__any_sync(0xffffffffu, m_new > m + kLazyGrowth)) {
-        carry = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - m_new);
-        m = m_new;
-        l *= carry;
-        rescale = true;
-      }
-      auto rescale_values = [&]() {
-#pragma unroll
-        for (int c = 0; c < D; c += 32) {
-          uint32_t o[32];
-          tile::ld32(o_tmem + c, o);
-          tile::wait_ld32(o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            o[i] = __float_as_uint(__uint_as_float(o[i]) * carry);
-          }
-          st32_tmem(o_tmem + c, o);
-        }
-      };
-      const float ref = m == -INFINITY ? 0.0f : m;
-      const f32x2 minus_ref = pack2(-ref, -ref);
-      f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-      if constexpr (!QUANT) {
-        if (rescale) {
-          rescale_values();
-        }
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t packed[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            float a, b;
-            unpack2(add2(pair_of(s + half * 64 + 2 * i), minus_ref), a, b);
-            a = fk_page_decode::exp2_quick(a);
-            b = fk_page_decode::exp2_quick(b);
-            sum[i & 1] = add2(sum[i & 1], pack2(a, b));
-            packed[i] = pack_bf16(a, b);
-          }
-          st32_tmem(s_tmem + 32 * half, packed);
-        }
-      } else {
-        // Weights are the probabilities times their token's value scale, brought to fp16's range by a
-        // power of two of the row's own, kept as lazily as the maximum.
-        const int index = 2 * j + 1;  // the scales come with the tile's values
+        const int index = 2 * j + 1;  // the value scales come with the tile's values
         ok = mbar_wait_parked(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
         if (!ok) {
           give_up();
           break;
         }
-        const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
+      }
+      const bool masked = (j + 1) * kTileTokens > unmasked[x];
+      const int seen = limit - j * kTileTokens;
+      uint32_t buffer[2][32];
+      // Logits of 32 tokens; with `masked` those that the row does not see are -inf.
+      auto take = [&](int c) {
+        uint32_t(&s)[32] = buffer[c & 1];
+        tile::wait_ld32(s);
+        if (c + 1 < 4) {
+          tile::ld32(s_tmem + 32 * (c + 1), buffer[(c + 1) & 1]);
+        }
+        if constexpr (QUANT) {
 #pragma unroll
-        for (int i = 0; i < 128; i += 4) {
-          const f32x2 f = pack2(factor[i / 16], factor[i / 16]);
-          const float4 v = value_factors[i / 4];
-#pragma unroll
-          for (int e = 0; e < 4; e += 2) {
+          for (int i = 0; i < 32; i += 2) {
             float a, b;
-            unpack2(fma2(pair_of(s + i + e), f, minus_ref), a, b);
-            a = fk_page_decode::exp2_quick(a);
-            b = fk_page_decode::exp2_quick(b);
-            const f32x2 prob = pack2(a, b);
-            sum[e / 2] = add2(sum[e / 2], prob);
-            unpack2(mul2(prob, e == 0 ? pack2(v.x, v.y) : pack2(v.z, v.w)), a, b);
-            s[i + e] = __float_as_uint(a);
-            s[i + e + 1] = __float_as_uint(b);
+            unpack2(mul2(pair_of(s + i), pack2(factor[2 * c + i / 16], factor[2 * c + i / 16])), a, b);
+            s[i] = __float_as_uint(a);
+            s[i + 1] = __float_as_uint(b);
           }
         }
-        const float heaviest = fmaxf(fmaxf(largest_of<32>(s), largest_of<32>(s + 32)), fmaxf(largest_of<32>(s + 64), largest_of<32>(s + 96)));
-        const int bits = fk_page_decode::exponent_bits(heaviest);
+        if (masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            s[i] = c * 32 + i < seen ? s[i] : 0xff800000u;
+          }
+        }
+      };
+      // ---- the tile's largest logit (QUANT: and the largest log2 of probability times value scale)
+      float top = m, heaviest = -INFINITY;
+      tile::ld32(s_tmem, buffer[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        take(c);
+        uint32_t(&s)[32] = buffer[c & 1];
+        top = fmaxf(top, largest_of<32>(s));
+        if constexpr (QUANT) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float4 v = value_logs[c * 8 + i / 4];
+            float a, b, e, f;
+            unpack2(add2(pair_of(s + i), pack2(v.x, v.y)), a, b);
+            unpack2(add2(pair_of(s + i + 2), pack2(v.z, v.w)), e, f);
+            heaviest = max3(heaviest, max3(a, b, e), f);
+          }
+        }
+      }
+      tile::ld32(s_tmem, buffer[0]);
+      float carry = 1.0f;  // what O is multiplied by
+      bool rescale = false;
+      if (j == 0) {
+        m = top;
+      } else if (__any_sync(0xffffffffu, top > m + kLazyGrowth)) {
+        carry = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - top);
+        m = top;
+        l *= carry;
+        rescale = true;
+      }
+      const float ref = m == -INFINITY ? 0.0f : m;
+      if constexpr (QUANT) {
+        // Weights are the probabilities times their token's value scale, brought to fp16's range by a
+        // power of two of the row's own, kept as lazily as the maximum.
+        const int bits = fk_page_decode::exponent_bits(fk_page_decode::exp2_quick(fminf(heaviest - ref, 120.0f)));
         if (j == 0) {
           o_bits = bits;
         } else if (rescale || __any_sync(0xffffffffu, bits > o_bits + (static_cast<int>(kLazyGrowth) << 23))) {
@@ -507,33 +474,66 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           carry = worth * fk_page_decode::inverse_power(o_bits);
           rescale = true;
         }
-        if (rescale) {
-          rescale_values();
-        }
-        const float shrink = fk_page_decode::inverse_power(o_bits);
-        const f32x2 shrink2 = pack2(shrink, shrink);
-#pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          uint32_t packed[32];
+      }
+      if (rescale) {
+        uint32_t o[32];
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          tile::ld32(o_tmem + c, o);
+          tile::wait_ld32(o);
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            float a, b;
-            unpack2(mul2(pair_of(s + half * 64 + 2 * i), shrink2), a, b);
-            packed[i] = pack_half(a, b);
+            o[i] = __float_as_uint(__uint_as_float(o[i]) * carry);
           }
-          st32_tmem(s_tmem + 32 * half, packed);
+          st32_tmem(o_tmem + c, o);
+        }
+      }
+      // ---- probabilities, over the logits' own columns: a half of the tile at a time, so that the
+      // ---- second product starts while the other half is still worked on
+      const f32x2 minus_ref = pack2(-ref, -ref);
+      const float shrink = fk_page_decode::inverse_power(o_bits);
+      const f32x2 shrink2 = pack2(shrink, shrink);
+      f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        take(c);
+        uint32_t(&s)[32] = buffer[c & 1];
+        uint32_t packed[16];
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          float a, b;
+          unpack2(add2(pair_of(s + i), minus_ref), a, b);
+          s[i] = __float_as_uint(fk_page_decode::exp2_quick(a));
+          s[i + 1] = __float_as_uint(fk_page_decode::exp2_quick(b));
+        }
+#pragma unroll
+        for (int i = 0; i < 32; i += 2) {
+          const f32x2 prob = pair_of(s + i);
+          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], prob);
+          float a, b;
+          if constexpr (QUANT) {
+            const float2 v = reinterpret_cast<const float2*>(value_factors)[c * 16 + i / 2];
+            unpack2(mul2(mul2(prob, pack2(v.x, v.y)), shrink2), a, b);
+            packed[i / 2] = pack_half(a, b);
+          } else {
+            unpack2(prob, a, b);
+            packed[i / 2] = pack_bf16(a, b);
+          }
+        }
+        umma::st16(s_tmem + 16 * c, packed);
+        if (c & 1) {
+          umma::wait_st();
+          umma::fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            umma::mbar_arrive(p_ready + 16 * (c >> 1) + 8 * x);
+          }
         }
       }
       {
         float a, b;
         unpack2(add2(sum[0], sum[1]), a, b);
         l += a + b;
-      }
-      umma::wait_st();
-      umma::fence_before_sync();
-      __syncwarp();
-      if (lane == 0) {
-        umma::mbar_arrive(p_ready + 8 * x);
       }
     }
     const float values_power = QUANT ? __int_as_float(o_bits) * (KV == kKvFp8 && kBlocks == 1 ? 256.0f : 1.0f) : 1.0f;
@@ -635,16 +635,21 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         }
         for (int x = 0; ok && x < 2; ++x) {
           if (j < tiles[x]) {
-            ok = mbar_wait_parked(p_ready + 8 * x, j & 1);
-            if (!ok) {
-              break;
-            }
-            umma::fence_after_sync();
             const uint64_t b = columns_desc(v_base);
 #pragma unroll
-            for (int k = 0; k < kTileTokens / 16; ++k) {
-              umma::mma_f16_ts(tmem + 256 + x * D, tmem + x * kTileTokens + 8 * k, b + k * (2048 >> 4), kValuesDesc,
-                               j == 0 && k == 0 ? 0u : 1u);
+            for (int half = 0; half < 2; ++half) {
+              ok = ok && mbar_wait_parked(p_ready + 16 * half + 8 * x, j & 1);
+              if (ok) {
+                umma::fence_after_sync();
+#pragma unroll
+                for (int k = 4 * half; k < 4 * half + 4; ++k) {
+                  umma::mma_f16_ts(tmem + 256 + x * D, tmem + x * kTileTokens + 8 * k, b + k * (2048 >> 4), kValuesDesc,
+                                   j == 0 && k == 0 ? 0u : 1u);
+                }
+              }
+            }
+            if (!ok) {
+              break;
             }
             if (j + 1 == tiles[x]) {
               umma::commit(o_final + 8 * x);
@@ -846,6 +851,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
             }
             if (chunk == 0) {
               factors[row] = larger;
+              factors[kFactorRing * kTileTokens + row] = __log2f(larger);
             }
             sts128(to + operand_chunk(row, chunk), out);
           }
