@@ -84,6 +84,22 @@ struct TcLayout {
   static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
 };
 
+// Bounded wait. The plain test comes first: most waits of the issuer and the copies are over when they
+// begin, and a test costs a few dozen clocks where try_wait takes some 150 even then.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(done)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return done != 0 || mbar_wait_parked(bar, parity);
+}
+
 __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                            uint32_t accumulate) {
   asm volatile(
@@ -293,62 +309,79 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       const int tasks = columns * slices;
       const int round = (tasks + 31) / 32 * 32;
       const int heads_each = (p.group + slices - 1) / slices;
+      constexpr int kBatch = 4;  // heads whose loads are in flight together
+      auto vector_of = [&](int task) -> int { return task < tasks ? (task / kChunks) % item.vectors : 0; };
+      int4 v = p.vectors[item.first_vector + vector_of(tid)];
       for (int task = tid; task < round; task += 256) {
         const bool active = task < tasks;
         const int chunk = task % kChunks;
-        const int vector = active ? (task / kChunks) % item.vectors : 0;
+        const int vector = vector_of(task);
         const int slice = active ? task / columns : 0;
-        const int4 v = p.vectors[item.first_vector + vector];
         const bool readable = active && v.x >= 0 && v.x < p.num_rows;
+        const int position = v.y;
+        const uint16_t* src = p.query + static_cast<long long>(readable ? v.x : 0) * p.query_row_stride +
+                              static_cast<long long>(item.kv_head * p.group) * p.query_head_stride + chunk * 8;
+        v = p.vectors[item.first_vector + vector_of(task + 256)];
         float2 cs[4];
+        for (int h0 = 0; h0 < heads_each; h0 += kBatch) {
+          uint4 w[kBatch];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float2 turn = rope_cos_sin(p.rope.turns[chunk * 4 + i], v.y);
-          cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
-        }
-        const uint16_t* src = p.query + static_cast<long long>(readable ? v.x : 0) * p.query_row_stride + chunk * 8;
-        for (int h = 0; h < heads_each; ++h) {
-          const int head = slice * heads_each + h;
-          const bool store = active && head < p.group;
-          uint4 w = make_uint4(0u, 0u, 0u, 0u);
-          if (store && readable) {
-            w = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(item.kv_head * p.group + head) *
-                                                              p.query_head_stride));
-          }
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
-          float q[8];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float even = bf16_low(words[i]), odd = bf16_high(words[i]);
-            q[2 * i] = even * cs[i].x - odd * cs[i].y;
-            q[2 * i + 1] = even * cs[i].y + odd * cs[i].x;
-          }
-          const int r = vector * p.group + head;
-          uint4 out;
-          if constexpr (QUANT) {
-            // fp16 has the precision but not the range: the row is divided by the power of two of its
-            // largest element, which goes back on in fp32
-            float largest = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              largest = fmaxf(largest, fabsf(q[i]));
+          for (int b = 0; b < kBatch; ++b) {
+            const int head = slice * heads_each + h0 + b;
+            w[b] = make_uint4(0u, 0u, 0u, 0u);
+            if (readable && h0 + b < heads_each && head < p.group) {
+              w[b] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(head) * p.query_head_stride));
             }
-#pragma unroll
-            for (int o = 1; o < kChunks; o <<= 1) {
-              largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
-            }
-            const int bits = fk_page_decode::exponent_bits(largest);
-            const float shrink = fk_page_decode::inverse_power(bits);
-            out = make_uint4(pack_half(q[0] * shrink, q[1] * shrink), pack_half(q[2] * shrink, q[3] * shrink),
-                             pack_half(q[4] * shrink, q[5] * shrink), pack_half(q[6] * shrink, q[7] * shrink));
-            if (store && chunk == 0) {
-              row_power[r] = __int_as_float(bits);
-            }
-          } else {
-            out = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
           }
-          if (store) {
-            sts128(base + L::kQueries + (r >> 7) * L::kOperandBytes + operand_chunk(r & 127, chunk), out);
+          if (h0 == 0) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 turn = rope_cos_sin(p.rope.turns[chunk * 4 + i], position);
+              cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            if (h0 + b >= heads_each) {
+              break;
+            }
+            const int head = slice * heads_each + h0 + b;
+            const bool store = active && head < p.group;
+            const uint32_t words[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
+            float q[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float even = bf16_low(words[i]), odd = bf16_high(words[i]);
+              q[2 * i] = even * cs[i].x - odd * cs[i].y;
+              q[2 * i + 1] = even * cs[i].y + odd * cs[i].x;
+            }
+            const int r = vector * p.group + head;
+            uint4 out;
+            if constexpr (QUANT) {
+              // fp16 has the precision but not the range: the row is divided by the power of two of its
+              // largest element, which goes back on in fp32
+              float largest = 0.0f;
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                largest = fmaxf(largest, fabsf(q[i]));
+              }
+#pragma unroll
+              for (int o = 1; o < kChunks; o <<= 1) {
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+              }
+              const int bits = fk_page_decode::exponent_bits(largest);
+              const float shrink = fk_page_decode::inverse_power(bits);
+              out = make_uint4(pack_half(q[0] * shrink, q[1] * shrink), pack_half(q[2] * shrink, q[3] * shrink),
+                               pack_half(q[4] * shrink, q[5] * shrink), pack_half(q[6] * shrink, q[7] * shrink));
+              if (store && chunk == 0) {
+                row_power[r] = __int_as_float(bits);
+              }
+            } else {
+              out = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
+            }
+            if (store) {
+              sts128(base + L::kQueries + (r >> 7) * L::kOperandBytes + operand_chunk(r & 127, chunk), out);
+            }
           }
         }
       }
@@ -381,7 +414,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     int o_bits = fk_page_decode::kMinExponentBits;  // QUANT: exponent bits of the power of two that O is divided by
     bool ok = true;
     for (int j = 0; j < tiles[x]; ++j) {
-      ok = mbar_wait_parked(s_ready + 8 * x, j & 1);
+      ok = wait_for(s_ready + 8 * x, j & 1);
       if (!ok) {
         give_up();
         break;
@@ -398,7 +431,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           factor[g] = factors[p.page_size == 16 ? g : g >> 1] * power;
         }
         const int index = 2 * j + 1;  // the value scales come with the tile's values
-        ok = mbar_wait_parked(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
+        ok = wait_for(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
         if (!ok) {
           give_up();
           break;
@@ -539,7 +572,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     const float values_power = QUANT ? __int_as_float(o_bits) * (KV == kKvFp8 && kBlocks == 1 ? 256.0f : 1.0f) : 1.0f;
     // ---- results --------------------------------------------------------------------------------
     const bool write_row = fits && r < rows && vec.x >= 0 && vec.x < p.num_rows;
-    if (tiles[x] > 0 && ok && !mbar_wait_parked(o_final + 8 * x, 0)) {
+    if (tiles[x] > 0 && ok && !wait_for(o_final + 8 * x, 0)) {
       give_up();
       ok = false;
     }
@@ -608,7 +641,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         }
         umma::commit(s_ready + 8 * x);
       };
-      bool ok = mbar_wait_parked(q_ready, 0) && mbar_wait_parked(full, 0);
+      bool ok = wait_for(q_ready, 0) && wait_for(full, 0);
       if (ok) {
         umma::fence_after_sync();
         for (int x = 0; x < 2; ++x) {
@@ -622,23 +655,21 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       for (int j = 0; ok && j < count; ++j) {
         const int v_slot = slot;
         const uint32_t v_base = base + L::kRing + v_slot * L::kOperandBytes;
-        ok = mbar_wait_parked(full + 8 * v_slot, slot_parity);
+        ok = wait_for(full + 8 * v_slot, slot_parity);
         if (ok && !QUANT && clear_needed && j == count - 1) {
           umma::mbar_arrive(v_landed);
-          ok = mbar_wait_parked(v_clear, 0);
+          ok = wait_for(v_clear, 0);
         }
         next_slot();
         const int k_slot = slot;
         const bool more = j + 1 < count;
-        if (ok && more) {
-          ok = mbar_wait_parked(full + 8 * k_slot, slot_parity);
-        }
+        bool k_there = false;
         for (int x = 0; ok && x < 2; ++x) {
           if (j < tiles[x]) {
             const uint64_t b = columns_desc(v_base);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              ok = ok && mbar_wait_parked(p_ready + 16 * half + 8 * x, j & 1);
+              ok = ok && wait_for(p_ready + 16 * half + 8 * x, j & 1);
               if (ok) {
                 umma::fence_after_sync();
 #pragma unroll
@@ -656,6 +687,14 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
             }
           }
           if (j + 1 < tiles[x]) {
+            if (!k_there) {
+              k_there = wait_for(full + 8 * k_slot, slot_parity);
+              if (!k_there) {
+                ok = false;
+                break;
+              }
+              umma::fence_after_sync();
+            }
             scores(x, base + L::kRing + k_slot * L::kOperandBytes);
           }
         }
@@ -709,7 +748,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         const int here = min(pages_per_tile, pages - j * pages_per_tile);  // pages of this tile
         for (int which = 0; which < 2; ++which) {  // keys, then values
           if (uses > 0) {
-            ok = mbar_wait_parked(bars_empty + 8 * slot, (uses - 1) & 1);
+            ok = wait_for(bars_empty + 8 * slot, (uses - 1) & 1);
             if (!ok) {
               break;
             }
@@ -766,7 +805,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         give_up();
         // let the copies in flight land before the shared memory is handed on
         for (int i = max(0, issued - kSlotCount); i < issued; ++i) {
-          if (!mbar_wait_parked(bars_full + 8 * (i % kSlotCount), (i / kSlotCount) & 1)) {
+          if (!wait_for(bars_full + 8 * (i % kSlotCount), (i / kSlotCount) & 1)) {
             break;
           }
         }
@@ -776,7 +815,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       // The issuer says when they have landed: it follows the ring's phases one by one, and a wait for
       // a later phase's parity would be over at once.
       const int slot = (2 * count - 1) % L::kSlots;  // the last tile's values, in the order of the copies
-      if (mbar_wait_parked(v_landed, 0)) {
+      if (wait_for(v_landed, 0)) {
         const int valid = loaded - (count - 1) * kTileTokens;
         const uint32_t v_base = base + L::kRing + slot * L::kOperandBytes;
         for (int idx = lane; idx < (kTileTokens - valid) * kChunks; idx += 32) {
@@ -796,6 +835,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       constexpr bool kShift = KV == kKvFp8;        // e4m3 numbers by bit operations, times 2^-8
       constexpr float kUnit = kShift ? 256.0f : 1.0f;
       const int t = tid - 384;
+      const int page_shift = p.page_size == 16 ? 4 : 5;
       const int chunk = t % kChunks;
       const int block = chunk / 8;
       int raw_slot = 0, slot = 0;
@@ -804,56 +844,90 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       for (int i = 0; ok && i < 2 * count; ++i) {
         const int j = i >> 1;
         const bool keys = (i & 1) == 0;
-        ok = mbar_wait_parked(raw_full + 8 * raw_slot, raw_uses & 1) &&
-             (uses == 0 || mbar_wait_parked(empty + 8 * slot, (uses - 1) & 1));
+        ok = wait_for(raw_full + 8 * raw_slot, raw_uses & 1) &&
+             (uses == 0 || wait_for(empty + 8 * slot, (uses - 1) & 1));
         if (!ok) {
           break;
         }
         const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
         const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
         const int valid = min(kTileTokens, loaded - j * kTileTokens);
+        // A thread's rows are first + pass * kRowsPerPass. Loads of several passes go out before the first
+        // store: the compiler may not move them across it.
+        constexpr int kPasses = kTileTokens / kRowsPerPass;
+        constexpr int kBatch = 8;
+        const int first = t / kChunks;
         if (keys) {
           const float2* scales = reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64);
           float* factors = reinterpret_cast<float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
-          if (t < kTileTokens / p.page_size) {
+          if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
             const float2 s = scales[t];
             factors[t] = fmaxf(s.x, s.y) * (kBlocks == 1 ? kUnit : 1.0f);
           }
-#pragma unroll 4
-          for (int row = t / kChunks; row < valid; row += kRowsPerPass) {
-            const uint2 w = lds64(from + row * D + chunk * 8);
-            uint4 out;
-            fk_page_decode::bytes_to_half2<KV, kShift>(w.x, out.x, out.y);
-            fk_page_decode::bytes_to_half2<KV, kShift>(w.y, out.z, out.w);
-            if constexpr (kBlocks == 2) {
-              const float2 s = scales[row / p.page_size];
-              scale_half8(out, block == 0 ? s.x : s.y, fmaxf(s.x, s.y), kUnit);
+#pragma unroll
+          for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
+            uint2 w[kBatch];
+            float2 s[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const int row = first + (pass0 + b) * kRowsPerPass;
+              w[b] = lds64(from + row * D + chunk * 8);
+              if constexpr (kBlocks == 2) {
+                s[b] = scales[row >> page_shift];
+              }
             }
-            sts128(to + operand_chunk(row, chunk), out);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const int row = first + (pass0 + b) * kRowsPerPass;
+              uint4 out;
+              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].x, out.x, out.y);
+              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].y, out.z, out.w);
+              if constexpr (kBlocks == 2) {
+                scale_half8(out, block == 0 ? s[b].x : s[b].y, fmaxf(s[b].x, s[b].y), kUnit);
+              }
+              sts128(to + operand_chunk(row, chunk), out);
+            }
           }
         } else {
           const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes);
           float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens;
-#pragma unroll 4
-          for (int row = t / kChunks; row < kTileTokens; row += kRowsPerPass) {
-            uint4 out = make_uint4(0u, 0u, 0u, 0u);
-            float larger = 0.0f;
-            if (row < valid) {
-              const uint2 w = lds64(from + row * D + chunk * 8);
-              fk_page_decode::bytes_to_half2<KV, kShift>(w.x, out.x, out.y);
-              fk_page_decode::bytes_to_half2<KV, kShift>(w.y, out.z, out.w);
-              larger = scales[row * kBlocks];
+          {
+            // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
+            float larger = scales[t * kBlocks];
+            if constexpr (kBlocks == 2) {
+              larger = fmaxf(larger, scales[t * kBlocks + 1]);
+            }
+            larger = t < valid ? larger : 0.0f;
+            factors[t] = larger;
+            factors[kFactorRing * kTileTokens + t] = __log2f(larger);
+          }
+#pragma unroll
+          for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
+            uint2 w[kBatch];
+            float2 s[kBatch];
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const int row = first + (pass0 + b) * kRowsPerPass;
+              w[b] = lds64(from + row * D + chunk * 8);
               if constexpr (kBlocks == 2) {
-                const float2 s = *reinterpret_cast<const float2*>(scales + row * 2);
-                larger = fmaxf(s.x, s.y);
-                scale_half8(out, block == 0 ? s.x : s.y, larger, kUnit);
+                s[b] = *reinterpret_cast<const float2*>(scales + row * 2);
               }
             }
-            if (chunk == 0) {
-              factors[row] = larger;
-              factors[kFactorRing * kTileTokens + row] = __log2f(larger);
+#pragma unroll
+            for (int b = 0; b < kBatch; ++b) {
+              const int row = first + (pass0 + b) * kRowsPerPass;
+              uint4 out;
+              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].x, out.x, out.y);
+              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].y, out.z, out.w);
+              if constexpr (kBlocks == 2) {
+                scale_half8(out, block == 0 ? s[b].x : s[b].y, fmaxf(s[b].x, s[b].y), kUnit);
+              }
+              // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
+              if (row >= valid) {
+                out = make_uint4(0u, 0u, 0u, 0u);
+              }
+              sts128(to + operand_chunk(row, chunk), out);
             }
-            sts128(to + operand_chunk(row, chunk), out);
           }
         }
         proxy_fence_async();
@@ -887,7 +961,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         umma::commit(drain);  // MMAs still in flight, if any
       }
       __syncwarp();
-      (void)mbar_wait_parked(drain, 0);
+      (void)wait_for(drain, 0);
     }
     umma::tmem_dealloc(tmem, 512);
   }
