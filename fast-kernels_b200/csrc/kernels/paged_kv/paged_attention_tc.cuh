@@ -79,7 +79,8 @@ struct TcLayout {
   static constexpr int kKeyFactors = kRaw + kRawSlots * kRawSlotBytes;              // [ring][8 pages]
   static constexpr int kValueFactors = kKeyFactors + (kQuant ? kFactorRing * 32 : 0);  // [ring][128 tokens], then their log2
   static constexpr int kRawKeyScales = kValueFactors + (kQuant ? kFactorRing * 1024 : 0);  // [raw slot][8 pages][2]
-  static constexpr int kRowPower = kRawKeyScales + kRawSlots * 64;                  // [256]
+  static constexpr int kRatios = kRawKeyScales + kRawSlots * 64;                    // [8 pages + 128 tokens][2]
+  static constexpr int kRowPower = kRatios + (kQuant ? 64 + 1024 : 0);              // [256]
   static constexpr int kBarriers = kRowPower + (kQuant ? 1024 : 0);
   static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
 };
@@ -183,16 +184,14 @@ __device__ __forceinline__ float largest_of(const uint32_t* r) {
   return max3(a, b, max3(a, __uint_as_float(r[N - 2]), __uint_as_float(r[N - 1])));
 }
 
-// Eight fp16 numbers times unit * mine / larger (exactly `unit` for the block that has the larger scale).
-// `unit` undoes the 2^-8 of shifted e4m3 numbers: what is left of the other block must stay clear of
-// fp16's subnormal numbers as far as it can.
-__device__ __forceinline__ void scale_half8(uint4& v, float mine, float larger, float unit) {
-  const __half2 ratio = __float2half2_rn(larger > 0.0f ? unit * __fdividef(mine, larger) : 0.0f);
-  __half2* h = reinterpret_cast<__half2*>(&v);
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    h[e] = __hmul2(h[e], ratio);
-  }
+// Two copies of mine / larger in fp16 (exactly 1 for the block that has the larger scale).
+__device__ __forceinline__ uint32_t scale_ratio(float mine, float larger) {
+  const __half2 ratio = __float2half2_rn(larger > 0.0f ? __fdividef(mine, larger) : 0.0f);
+  return *reinterpret_cast<const uint32_t*>(&ratio);
+}
+__device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
+  const __half2 product = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+  return *reinterpret_cast<const uint32_t*>(&product);
 }
 
 template <int D, int KV>
@@ -569,7 +568,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         l += a + b;
       }
     }
-    const float values_power = QUANT ? __int_as_float(o_bits) * (KV == kKvFp8 && kBlocks == 1 ? 256.0f : 1.0f) : 1.0f;
+    const float values_power = QUANT ? __int_as_float(o_bits) : 1.0f;
     // ---- results --------------------------------------------------------------------------------
     const bool write_row = fits && r < rows && vec.x >= 0 && vec.x < p.num_rows;
     if (tiles[x] > 0 && ok && !wait_for(o_final + 8 * x, 0)) {
@@ -832,12 +831,18 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     } else if (QUANT && warp >= 12 && count > 0) {
       // ---- 8-bit tiles to 16 bits ---------------------------------------------------------------
       constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
-      constexpr bool kShift = KV == kKvFp8;        // e4m3 numbers by bit operations, times 2^-8
-      constexpr float kUnit = kShift ? 256.0f : 1.0f;
+      constexpr int kPasses = kTileTokens / kRowsPerPass;
+      // A thread's rows are first + pass * kRowsPerPass, a batch at a time: all loads, all arithmetic, all
+      // stores. (The loads and stores are volatile: in the order of one row after the other every row
+      // waits for the one before, 230 clocks each.)
+      constexpr int kBatch = 4;
+      uint32_t* key_ratios = reinterpret_cast<uint32_t*>(smem + L::kRatios);  // [8 pages][2 blocks]
+      uint32_t* value_ratios = key_ratios + 16;                               // [128 rows][2 blocks]
       const int t = tid - 384;
       const int page_shift = p.page_size == 16 ? 4 : 5;
       const int chunk = t % kChunks;
       const int block = chunk / 8;
+      const int first = t / kChunks;
       int raw_slot = 0, slot = 0;
       uint32_t raw_uses = 0, uses = 0;
       bool ok = true;
@@ -852,82 +857,63 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
         const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
         const int valid = min(kTileTokens, loaded - j * kTileTokens);
-        // A thread's rows are first + pass * kRowsPerPass. Loads of several passes go out before the first
-        // store: the compiler may not move them across it.
-        constexpr int kPasses = kTileTokens / kRowsPerPass;
-        constexpr int kBatch = 8;
-        const int first = t / kChunks;
+        const uint32_t* ratios = keys ? key_ratios : value_ratios;
         if (keys) {
-          const float2* scales = reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64);
-          float* factors = reinterpret_cast<float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
           if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
-            const float2 s = scales[t];
-            factors[t] = fmaxf(s.x, s.y) * (kBlocks == 1 ? kUnit : 1.0f);
-          }
-#pragma unroll
-          for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
-            uint2 w[kBatch];
-            float2 s[kBatch];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-              const int row = first + (pass0 + b) * kRowsPerPass;
-              w[b] = lds64(from + row * D + chunk * 8);
-              if constexpr (kBlocks == 2) {
-                s[b] = scales[row >> page_shift];
-              }
-            }
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-              const int row = first + (pass0 + b) * kRowsPerPass;
-              uint4 out;
-              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].x, out.x, out.y);
-              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].y, out.z, out.w);
-              if constexpr (kBlocks == 2) {
-                scale_half8(out, block == 0 ? s[b].x : s[b].y, fmaxf(s[b].x, s[b].y), kUnit);
-              }
-              sts128(to + operand_chunk(row, chunk), out);
+            const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + t * 8);
+            const float larger = fmaxf(s.x, s.y);
+            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + t] = larger;
+            if constexpr (kBlocks == 2) {
+              key_ratios[2 * t] = scale_ratio(s.x, larger);
+              key_ratios[2 * t + 1] = scale_ratio(s.y, larger);
             }
           }
         } else {
-          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes);
-          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens;
-          {
-            // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
-            float larger = scales[t * kBlocks];
-            if constexpr (kBlocks == 2) {
-              larger = fmaxf(larger, scales[t * kBlocks + 1]);
-            }
-            larger = t < valid ? larger : 0.0f;
-            factors[t] = larger;
-            factors[kFactorRing * kTileTokens + t] = __log2f(larger);
+          // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
+          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes) + t * kBlocks;
+          float larger = scales[0];
+          if constexpr (kBlocks == 2) {
+            larger = fmaxf(larger, scales[1]);
+            value_ratios[2 * t] = scale_ratio(scales[0], larger);
+            value_ratios[2 * t + 1] = scale_ratio(scales[1], larger);
+          }
+          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
+          factors[0] = t < valid ? larger : 0.0f;
+          factors[kFactorRing * kTileTokens] = t < valid ? __log2f(larger) : -INFINITY;
+        }
+        if constexpr (kBlocks == 2) {
+          asm volatile("bar.sync 2, 128;" ::: "memory");  // the ratios, by the rows' other threads
+        }
+#pragma unroll
+        for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
+          uint2 w[kBatch];
+          uint32_t ratio[kBatch];
+          uint4 out[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = first + (pass0 + b) * kRowsPerPass;
+            w[b] = lds64(from + row * D + chunk * 8);
+            ratio[b] = kBlocks == 2 ? ratios[(keys ? row >> page_shift : row) * 2 + block] : 0u;
           }
 #pragma unroll
-          for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
-            uint2 w[kBatch];
-            float2 s[kBatch];
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-              const int row = first + (pass0 + b) * kRowsPerPass;
-              w[b] = lds64(from + row * D + chunk * 8);
-              if constexpr (kBlocks == 2) {
-                s[b] = *reinterpret_cast<const float2*>(scales + row * 2);
-              }
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = first + (pass0 + b) * kRowsPerPass;
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out[b].x, out[b].y);
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out[b].z, out[b].w);
+            if constexpr (kBlocks == 2) {
+              out[b].x = mul_half2(out[b].x, ratio[b]);
+              out[b].y = mul_half2(out[b].y, ratio[b]);
+              out[b].z = mul_half2(out[b].z, ratio[b]);
+              out[b].w = mul_half2(out[b].w, ratio[b]);
             }
-#pragma unroll
-            for (int b = 0; b < kBatch; ++b) {
-              const int row = first + (pass0 + b) * kRowsPerPass;
-              uint4 out;
-              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].x, out.x, out.y);
-              fk_page_decode::bytes_to_half2<KV, kShift>(w[b].y, out.z, out.w);
-              if constexpr (kBlocks == 2) {
-                scale_half8(out, block == 0 ? s[b].x : s[b].y, fmaxf(s[b].x, s[b].y), kUnit);
-              }
-              // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
-              if (row >= valid) {
-                out = make_uint4(0u, 0u, 0u, 0u);
-              }
-              sts128(to + operand_chunk(row, chunk), out);
+            // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
+            if (row >= valid) {
+              out[b] = make_uint4(0u, 0u, 0u, 0u);
             }
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            sts128(to + operand_chunk(first + (pass0 + b) * kRowsPerPass, chunk), out[b]);
           }
         }
         proxy_fence_async();
