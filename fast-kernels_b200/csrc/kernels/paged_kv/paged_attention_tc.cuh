@@ -15,9 +15,12 @@
 // overlap one exponential with the next.
 //
 // The running maximum is kept lazily: O is multiplied by 2^(old - new) only when a row's maximum has
-// grown by more than 2^8 since the last time, else P may be up to 2^8 and nothing is lost (bf16 and
-// fp32 have the range). The tensor core is done with O whenever a tile's logits are: their commit
-// follows the previous tile's second product.
+// grown by more than kGrowth since the last time. The tensor core is done with O whenever a tile's logits
+// are: their commit follows the previous tile's second product.
+//
+// The exponentials are what the softmax warps are bound by (16 a clock and SM: 2048 clocks per token tile
+// and 256 rows, the two products take as long). With bf16 pages a quarter of them, in tiles without a
+// mask, is a polynomial on the FMA pipe.
 //
 // Roles (warps): 0-3 and 4-7 softmax of the two row tiles (they also turn and store the queries, and
 // write the results), 8 issues the MMAs, 9 the copies, 10 clears the value rows behind the end (a
@@ -33,6 +36,8 @@
 #pragma once
 
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "../clustered_page_decode/page_decode_kernel.cuh"
 #include "../decode_quant_linear/w4a16_gemm_tile.cuh"
@@ -53,7 +58,6 @@ using fk_w4a16::smem_addr;
 constexpr int kTileRows = 128;
 constexpr int kTileTokens = 128;
 constexpr int kFactorRing = 4;  // token tiles whose scales are kept for the softmax warps
-constexpr float kLazyGrowth = 8.0f;
 constexpr int kStatusWaitTimeout = 1;
 
 template <int D, int KV>
@@ -80,7 +84,8 @@ struct TcLayout {
   static constexpr int kValueFactors = kKeyFactors + (kQuant ? kFactorRing * 32 : 0);  // [ring][128 tokens], then their log2
   static constexpr int kRawKeyScales = kValueFactors + (kQuant ? kFactorRing * 1024 : 0);  // [raw slot][8 pages][2]
   static constexpr int kRatios = kRawKeyScales + kRawSlots * 64;                    // [8 pages + 128 tokens][2]
-  static constexpr int kRowPower = kRatios + (kQuant ? 64 + 1024 : 0);              // [256]
+  static constexpr int kTileLogs = kRatios + (kQuant ? 64 + 1024 : 0);              // [ring][4 warps]
+  static constexpr int kRowPower = kTileLogs + (kQuant ? kFactorRing * 16 : 0);     // [256]
   static constexpr int kBarriers = kRowPower + (kQuant ? 1024 : 0);
   static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
 };
@@ -184,6 +189,27 @@ __device__ __forceinline__ float largest_of(const uint32_t* r) {
   return max3(a, b, max3(a, __uint_as_float(r[N - 2]), __uint_as_float(r[N - 1])));
 }
 
+// 2^x for two x <= 8 on the FMA pipe: x = i + f, |f| <= 1/2, a polynomial of degree 4 in f (minimax for the
+// relative error, by Remez exchange: 2^-18.5) and i added to the exponent. Below -126 the result is about
+// 2^-126 instead of less.
+__device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
+  float a, b;
+  unpack2(x, a, b);
+  x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+  const f32x2 magic = pack2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's last bits are round(x)
+  const f32x2 shifted = add2(x, magic);
+  const f32x2 f = add2(x, fma2(shifted, pack2(-1.0f, -1.0f), magic));
+  f32x2 r = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
+  r = fma2(r, f, pack2(0.240247443318367f, 0.240247443318367f));
+  r = fma2(r, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+  r = fma2(r, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+  float ra, rb, sa, sb;
+  unpack2(r, ra, rb);
+  unpack2(shifted, sa, sb);
+  return pack2(__int_as_float(__float_as_int(ra) + (__float_as_int(sa) << 23)),
+               __int_as_float(__float_as_int(rb) + (__float_as_int(sb) << 23)));
+}
+
 // Two copies of mine / larger in fp16 (exactly 1 for the block that has the larger scale).
 __device__ __forceinline__ uint32_t scale_ratio(float mine, float larger) {
   const __half2 ratio = __float2half2_rn(larger > 0.0f ? __fdividef(mine, larger) : 0.0f);
@@ -202,6 +228,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   constexpr bool QUANT = L::kQuant;
   constexpr int kBlocks = D / 64;          // scale blocks, and halves of an operand
   constexpr int kChunks = D / 8;           // 16-byte chunks of a row
+  // How far a row's largest probability (weight) may be above 1, as a power of two, before O is rescaled:
+  // 8-bit pages, fp16 weights: below 2^16; bf16 has the range, and O should not lose it.
+  constexpr float kGrowth = QUANT ? 15.0f : 8.0f;
   constexpr uint32_t kScoresDesc = instruction_desc(!QUANT, kTileTokens, false);
   constexpr uint32_t kValuesDesc = instruction_desc(!QUANT, D, true);
   extern __shared__ __align__(16) uint8_t raw_smem[];
@@ -409,8 +438,10 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     const int4 vec = fits ? p.vectors[item.first_vector + my_vector] : make_int4(0, 0, 0, 0);
     const int limit = (item.causal != 0 ? min(item.end_token, vec.y + 1) : item.end_token) - item.first_token;
     const float power = QUANT && count > 0 ? row_power[r] : 1.0f;
+    // `m` is what probabilities are relative to, 2^(logit - m). bf16 pages: the largest logit (kept lazily).
+    // 8-bit pages: the largest logit + log2 of the token's value scale, that is the heaviest weight
+    // (probability times scale), which is what has to stay within fp16.
     float m = -INFINITY, l = 0.0f;
-    int o_bits = fk_page_decode::kMinExponentBits;  // QUANT: exponent bits of the power of two that O is divided by
     bool ok = true;
     for (int j = 0; j < tiles[x]; ++j) {
       ok = wait_for(s_ready + 8 * x, j & 1);
@@ -419,6 +450,8 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         break;
       }
       umma::fence_after_sync();
+      const bool masked = (j + 1) * kTileTokens > unmasked[x];
+      const int seen = limit - j * kTileTokens;
       // QUANT: what 16 neighbouring logits are multiplied by, the page's key scale and the row's power of two
       float factor[8];
       const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
@@ -429,85 +462,76 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         for (int g = 0; g < 8; ++g) {
           factor[g] = factors[p.page_size == 16 ? g : g >> 1] * power;
         }
+      }
+      uint32_t buffer[2][32];
+      // Products of 32 tokens; with `masked` the logits, -inf where the row does not see the token.
+      auto take = [&](int c, auto all_seen) {
+        uint32_t(&s)[32] = buffer[c & 1];
+        tile::wait_ld32(s);
+        if (c + 1 < 4) {
+          tile::ld32(s_tmem + 32 * (c + 1), buffer[(c + 1) & 1]);
+        }
+        if (!decltype(all_seen)::value && masked) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            const float logit = QUANT ? __uint_as_float(s[i]) * factor[2 * c + i / 16] : __uint_as_float(s[i]);
+            s[i] = c * 32 + i < seen ? __float_as_uint(logit) : 0xff800000u;
+          }
+        }
+      };
+      auto factor_of = [&](int g) -> float { return masked ? 1.0f : factor[g]; };
+      // ---- the tile's largest logit ----
+      float top = -INFINITY;
+      tile::ld32(s_tmem, buffer[0]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        take(c, std::false_type{});
+        uint32_t(&s)[32] = buffer[c & 1];
+        if constexpr (QUANT) {  // (scales are not negative)
+          top = max3(top, largest_of<16>(s) * factor_of(2 * c), largest_of<16>(s + 16) * factor_of(2 * c + 1));
+        } else {
+          top = fmaxf(top, largest_of<32>(s));
+        }
+      }
+      if constexpr (QUANT) {
         const int index = 2 * j + 1;  // the value scales come with the tile's values
         ok = wait_for(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
         if (!ok) {
           give_up();
           break;
         }
-      }
-      const bool masked = (j + 1) * kTileTokens > unmasked[x];
-      const int seen = limit - j * kTileTokens;
-      uint32_t buffer[2][32];
-      // Logits of 32 tokens; with `masked` those that the row does not see are -inf.
-      auto take = [&](int c) {
-        uint32_t(&s)[32] = buffer[c & 1];
-        tile::wait_ld32(s);
-        if (c + 1 < 4) {
-          tile::ld32(s_tmem + 32 * (c + 1), buffer[(c + 1) & 1]);
-        }
-        if constexpr (QUANT) {
+        const float4 logs = reinterpret_cast<const float4*>(smem + L::kTileLogs)[j % kFactorRing];
+        const float bound = top + fmaxf(fmaxf(logs.x, logs.y), fmaxf(logs.z, logs.w));
+        if (j == 0 || __any_sync(0xffffffffu, bound > m + kGrowth)) {
+          // the heaviest weight itself: the bound may be far above it
+          top = -INFINITY;
+          tile::ld32(s_tmem, buffer[0]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            float a, b;
-            unpack2(mul2(pair_of(s + i), pack2(factor[2 * c + i / 16], factor[2 * c + i / 16])), a, b);
-            s[i] = __float_as_uint(a);
-            s[i + 1] = __float_as_uint(b);
+          for (int c = 0; c < 4; ++c) {
+            take(c, std::false_type{});
+            uint32_t(&s)[32] = buffer[c & 1];
+#pragma unroll
+            for (int i = 0; i < 32; i += 4) {
+              const f32x2 f = pack2(factor_of(2 * c + i / 16), factor_of(2 * c + i / 16));
+              const float4 v = value_logs[c * 8 + i / 4];
+              float a, b, e, g;
+              unpack2(fma2(pair_of(s + i), f, pack2(v.x, v.y)), a, b);
+              unpack2(fma2(pair_of(s + i + 2), f, pack2(v.z, v.w)), e, g);
+              top = max3(top, max3(a, b, e), g);
+            }
           }
-        }
-        if (masked) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            s[i] = c * 32 + i < seen ? s[i] : 0xff800000u;
-          }
-        }
-      };
-      // ---- the tile's largest logit (QUANT: and the largest log2 of probability times value scale)
-      float top = m, heaviest = -INFINITY;
-      tile::ld32(s_tmem, buffer[0]);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        take(c);
-        uint32_t(&s)[32] = buffer[c & 1];
-        top = fmaxf(top, largest_of<32>(s));
-        if constexpr (QUANT) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            const float4 v = value_logs[c * 8 + i / 4];
-            float a, b, e, f;
-            unpack2(add2(pair_of(s + i), pack2(v.x, v.y)), a, b);
-            unpack2(add2(pair_of(s + i + 2), pack2(v.z, v.w)), e, f);
-            heaviest = max3(heaviest, max3(a, b, e), f);
-          }
+        } else {
+          top = m;
         }
       }
       tile::ld32(s_tmem, buffer[0]);
-      float carry = 1.0f;  // what O is multiplied by
-      bool rescale = false;
       if (j == 0) {
         m = top;
-      } else if (__any_sync(0xffffffffu, top > m + kLazyGrowth)) {
-        carry = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - top);
-        m = top;
+      } else if (__any_sync(0xffffffffu, top > m + (QUANT ? 0.0f : kGrowth))) {
+        const float m_new = fmaxf(m, top);
+        const float carry = m == -INFINITY ? 0.0f : fk_page_decode::exp2_quick(m - m_new);
+        m = m_new;
         l *= carry;
-        rescale = true;
-      }
-      const float ref = m == -INFINITY ? 0.0f : m;
-      if constexpr (QUANT) {
-        // Weights are the probabilities times their token's value scale, brought to fp16's range by a
-        // power of two of the row's own, kept as lazily as the maximum.
-        const int bits = fk_page_decode::exponent_bits(fk_page_decode::exp2_quick(fminf(heaviest - ref, 120.0f)));
-        if (j == 0) {
-          o_bits = bits;
-        } else if (rescale || __any_sync(0xffffffffu, bits > o_bits + (static_cast<int>(kLazyGrowth) << 23))) {
-          // the power follows what the old sum is worth under the new maximum, up or down
-          const float worth = __int_as_float(o_bits) * carry;
-          o_bits = max(bits, fk_page_decode::exponent_bits(worth));
-          carry = worth * fk_page_decode::inverse_power(o_bits);
-          rescale = true;
-        }
-      }
-      if (rescale) {
         uint32_t o[32];
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
@@ -522,34 +546,59 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       }
       // ---- probabilities, over the logits' own columns: a half of the tile at a time, so that the
       // ---- second product starts while the other half is still worked on
+      const float ref = m == -INFINITY ? 0.0f : m;
       const f32x2 minus_ref = pack2(-ref, -ref);
-      const float shrink = fk_page_decode::inverse_power(o_bits);
-      const f32x2 shrink2 = pack2(shrink, shrink);
       f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+      auto probabilities = [&](auto all_seen) {  // in two instances: the compiler leaves the branch in otherwise
+        constexpr bool kAllSeen = decltype(all_seen)::value;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        take(c);
+        take(c, all_seen);
         uint32_t(&s)[32] = buffer[c & 1];
         uint32_t packed[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
+          f32x2 e;
+          if constexpr (QUANT) {
+            const float f = kAllSeen ? factor[2 * c + i / 16] : 1.0f;
+            e = fma2(pair_of(s + i), pack2(f, f), minus_ref);
+          } else {
+            e = add2(pair_of(s + i), minus_ref);
+          }
           float a, b;
-          unpack2(add2(pair_of(s + i), minus_ref), a, b);
-          s[i] = __float_as_uint(fk_page_decode::exp2_quick(a));
-          s[i + 1] = __float_as_uint(fk_page_decode::exp2_quick(b));
+          if constexpr (!QUANT && kAllSeen) {
+            if (i % 8 == 6) {
+              unpack2(exp2_pair(e), a, b);
+            } else {
+              unpack2(e, a, b);
+              a = fk_page_decode::exp2_quick(a);
+              b = fk_page_decode::exp2_quick(b);
+            }
+          } else {
+            unpack2(e, a, b);
+            a = fk_page_decode::exp2_quick(a);
+            b = fk_page_decode::exp2_quick(b);
+          }
+          s[i] = __float_as_uint(a);
+          s[i + 1] = __float_as_uint(b);
         }
 #pragma unroll
-        for (int i = 0; i < 32; i += 2) {
-          const f32x2 prob = pair_of(s + i);
-          sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], prob);
+        for (int i = 0; i < 32; i += 4) {
+          const f32x2 first = pair_of(s + i), second = pair_of(s + i + 2);
+          sum[0] = add2(sum[0], first);
+          sum[1] = add2(sum[1], second);
           float a, b;
           if constexpr (QUANT) {
-            const float2 v = reinterpret_cast<const float2*>(value_factors)[c * 16 + i / 2];
-            unpack2(mul2(mul2(prob, pack2(v.x, v.y)), shrink2), a, b);
+            const float4 v = value_factors[c * 8 + i / 4];
+            unpack2(mul2(first, pack2(v.x, v.y)), a, b);
             packed[i / 2] = pack_half(a, b);
+            unpack2(mul2(second, pack2(v.z, v.w)), a, b);
+            packed[i / 2 + 1] = pack_half(a, b);
           } else {
-            unpack2(prob, a, b);
+            unpack2(first, a, b);
             packed[i / 2] = pack_bf16(a, b);
+            unpack2(second, a, b);
+            packed[i / 2 + 1] = pack_bf16(a, b);
           }
         }
         umma::st16(s_tmem + 16 * c, packed);
@@ -562,13 +611,18 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           }
         }
       }
+      };
+      if (masked) {
+        probabilities(std::false_type{});
+      } else {
+        probabilities(std::true_type{});
+      }
       {
         float a, b;
         unpack2(add2(sum[0], sum[1]), a, b);
         l += a + b;
       }
     }
-    const float values_power = QUANT ? __int_as_float(o_bits) : 1.0f;
     // ---- results --------------------------------------------------------------------------------
     const bool write_row = fits && r < rows && vec.x >= 0 && vec.x < p.num_rows;
     if (tiles[x] > 0 && ok && !wait_for(o_final + 8 * x, 0)) {
@@ -579,7 +633,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       umma::fence_after_sync();
       const bool direct = item.partial < 0;
       const bool slot_fits = direct || (item.partial < vec.w && vec.z >= 0 && vec.z + item.partial < p.num_partials);
-      const float inv = l == 0.0f ? 0.0f : values_power / l;
+      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
       uint16_t* out = p.output + (static_cast<size_t>(vec.x) * p.num_q_heads + my_head) * D;
       float* part = p.partials + (static_cast<size_t>(vec.z + item.partial) * p.num_q_heads + my_head) * (D + 4);
 #pragma unroll
@@ -607,9 +661,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           } else {
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
-              *reinterpret_cast<float4*>(part + c + i) =
-                  make_float4(__uint_as_float(o[i]) * values_power, __uint_as_float(o[i + 1]) * values_power,
-                              __uint_as_float(o[i + 2]) * values_power, __uint_as_float(o[i + 3]) * values_power);
+              *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
             }
           }
         }
@@ -879,7 +931,17 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           }
           float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
           factors[0] = t < valid ? larger : 0.0f;
-          factors[kFactorRing * kTileTokens] = t < valid ? __log2f(larger) : -INFINITY;
+          // (a scale of 0 must not leave a tile without a finite heaviest weight)
+          const float log = t < valid ? __log2f(fmaxf(larger, 1e-30f)) : -INFINITY;
+          factors[kFactorRing * kTileTokens] = log;
+          float most = log;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          }
+          if (lane == 0) {
+            reinterpret_cast<float*>(smem + L::kTileLogs)[(j % kFactorRing) * 4 + (warp & 3)] = most;
+          }
         }
         if constexpr (kBlocks == 2) {
           asm volatile("bar.sync 2, 128;" ::: "memory");  // the ratios, by the rows' other threads
