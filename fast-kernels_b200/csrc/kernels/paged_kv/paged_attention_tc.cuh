@@ -23,7 +23,7 @@
 // mask, is a polynomial on the FMA pipe.
 //
 // Roles (warps): 0-3 and 4-7 softmax of the two row tiles (they also turn and store the queries, and
-// write the results), 8 issues the MMAs, 9 the copies, 10 clears the value rows behind the end (a
+// write the results), 8 and 11 issue the two tiles' MMAs, 9 the copies, 10 clears the value rows behind the end (a
 // probability of 0 times whatever a page holds there would not be 0). 8-bit pages: 12-15 convert.
 // Every wait is bounded.
 //
@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   // both, a late issuer would find its phase overtaken by the next.
   const uint32_t p_ready = bars + 352;
   const uint32_t o_final = bars + 56;             // [2] the last product is done
+  const uint32_t turn = bars + 384;               // [2] the tile's issuer may issue
   const uint32_t v_clear = bars + 72;
   const uint32_t drain = bars + 80;
   const uint32_t v_landed = bars + 88;
@@ -265,13 +266,14 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       mbar_init(p_ready + 8 * x, 4);
       mbar_init(p_ready + 16 + 8 * x, 4);
       mbar_init(o_final + 8 * x, 1);
+      mbar_init(turn + 8 * x, 1);
     }
     mbar_init(v_landed, 1);
     mbar_init(v_clear, 1);
-    mbar_init(drain, 1);
+    mbar_init(drain, 2);
     for (int s = 0; s < L::kSlots; ++s) {
       mbar_init(full + 8 * s, QUANT ? 4 : 1);
-      mbar_init(empty + 8 * s, 1);
+      mbar_init(empty + 8 * s, 2);
     }
     for (int s = 0; s < L::kRawSlots; ++s) {
       mbar_init(raw_full + 8 * s, 1);
@@ -672,89 +674,88 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     }
   } else {
     tile::registers_down<L::kOtherRegisters>();
-    if (warp == 8 && lane == 0 && count > 0) {
-      // ---- MMA issuer ---------------------------------------------------------------------------
-      int slot = 0;
-      uint32_t slot_parity = 0;
-      auto next_slot = [&]() {
-        if (++slot == L::kSlots) {
-          slot = 0;
-          slot_parity ^= 1u;
+    if ((warp == 8 || warp == 11) && lane == 0 && count > 0) {
+      // ---- MMA issuers --------------------------------------------------------------------------
+      // One per row tile, taking turns: while one issues O_X += P_X(j) V(j) and, behind it, S_X(j + 1) over
+      // P_X(j)'s columns, the other goes through its waits and commits. (A single issuer left the tensor
+      // core idle for 700 of 3450 clocks a token tile; without the turns the two row tiles' products run,
+      // and end, at the same time, and so do the exponentials that wait for them: 707 us for 628.)
+      const int x = warp == 8 ? 0 : 1;
+      const int mine = tiles[x];
+      auto slot_of = [&](int index) -> uint32_t { return index % L::kSlots; };  // keys 2 j, values 2 j + 1
+      auto landed = [&](int index) -> bool { return wait_for(full + 8 * slot_of(index), (index / L::kSlots) & 1); };
+      auto release = [&](int index, bool used) {
+        if (used) {
+          umma::commit(empty + 8 * slot_of(index));
+        } else {
+          umma::mbar_arrive(empty + 8 * slot_of(index));
         }
       };
-      auto scores = [&](int x, uint32_t k_base) {
-        const uint64_t a = rows_desc(base + L::kQueries + x * L::kOperandBytes);
-        const uint64_t b = rows_desc(k_base);
+      // Row tile 0 begins; a turn's end is an arrival at the other's barrier.
+      auto wait_turn = [&](int n) -> bool { return wait_for(turn + 8 * x, (n & 1) ^ (x == 0 ? 1 : 0)); };
+      auto end_turn = [&]() { umma::mbar_arrive(turn + 8 * (1 - x)); };
+      const uint64_t queries = rows_desc(base + L::kQueries + x * L::kOperandBytes);
+      auto scores = [&](int j) {
+        const uint64_t b = rows_desc(base + L::kRing + slot_of(2 * j) * L::kOperandBytes);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k) {
           const uint64_t step = static_cast<uint64_t>((k / 4) * (L::kHalfBytes >> 4) + (k % 4) * 2);
-          mma_f16_ss(tmem + x * kTileTokens, a + step, b + step, kScoresDesc, k == 0 ? 0u : 1u);
+          mma_f16_ss(tmem + x * kTileTokens, queries + step, b + step, kScoresDesc, k == 0 ? 0u : 1u);
         }
         umma::commit(s_ready + 8 * x);
       };
-      bool ok = wait_for(q_ready, 0) && wait_for(full, 0);
+      bool ok = wait_for(q_ready, 0) && landed(0) && wait_turn(0);
       if (ok) {
-        umma::fence_after_sync();
-        for (int x = 0; x < 2; ++x) {
-          if (tiles[x] > 0) {
-            scores(x, base + L::kRing);
-          }
+        if (mine > 0) {
+          umma::fence_after_sync();
+          scores(0);
         }
-        umma::commit(empty);
-        next_slot();
+        end_turn();
+        release(0, mine > 0);
       }
       for (int j = 0; ok && j < count; ++j) {
-        const int v_slot = slot;
-        const uint32_t v_base = base + L::kRing + v_slot * L::kOperandBytes;
-        ok = wait_for(full + 8 * v_slot, slot_parity);
-        if (ok && !QUANT && clear_needed && j == count - 1) {
-          umma::mbar_arrive(v_landed);
+        const bool more = j + 1 < count;
+        ok = landed(2 * j + 1);
+        if (ok && !QUANT && clear_needed && !more) {
+          if (x == 0) {
+            umma::mbar_arrive(v_landed);
+          }
           ok = wait_for(v_clear, 0);
         }
-        next_slot();
-        const int k_slot = slot;
-        const bool more = j + 1 < count;
-        bool k_there = false;
-        for (int x = 0; ok && x < 2; ++x) {
-          if (j < tiles[x]) {
-            const uint64_t b = columns_desc(v_base);
+        ok = ok && (!more || landed(2 * j + 2));
+        if (ok && j < mine) {
+          ok = wait_for(p_ready + 8 * x, j & 1);
+        }
+        ok = ok && wait_turn(j + 1);
+        if (!ok) {
+          break;
+        }
+        if (j < mine) {
+          const uint64_t b = columns_desc(base + L::kRing + slot_of(2 * j + 1) * L::kOperandBytes);
+          auto values = [&](int half) {
+            umma::fence_after_sync();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              ok = ok && wait_for(p_ready + 16 * half + 8 * x, j & 1);
-              if (ok) {
-                umma::fence_after_sync();
-#pragma unroll
-                for (int k = 4 * half; k < 4 * half + 4; ++k) {
-                  umma::mma_f16_ts(tmem + 256 + x * D, tmem + x * kTileTokens + 8 * k, b + k * (2048 >> 4), kValuesDesc,
-                                   j == 0 && k == 0 ? 0u : 1u);
-                }
-              }
+            for (int k = 4 * half; k < 4 * half + 4; ++k) {
+              umma::mma_f16_ts(tmem + 256 + x * D, tmem + x * kTileTokens + 8 * k, b + k * (2048 >> 4), kValuesDesc,
+                               j == 0 && k == 0 ? 0u : 1u);
             }
-            if (!ok) {
-              break;
-            }
-            if (j + 1 == tiles[x]) {
-              umma::commit(o_final + 8 * x);
-            }
+          };
+          values(0);
+          ok = wait_for(p_ready + 16 + 8 * x, j & 1);
+          if (!ok) {
+            break;
           }
-          if (j + 1 < tiles[x]) {
-            if (!k_there) {
-              k_there = wait_for(full + 8 * k_slot, slot_parity);
-              if (!k_there) {
-                ok = false;
-                break;
-              }
-              umma::fence_after_sync();
-            }
-            scores(x, base + L::kRing + k_slot * L::kOperandBytes);
+          values(1);
+          if (j + 1 < mine) {
+            scores(j + 1);
+          } else {
+            umma::commit(o_final + 8 * x);
           }
         }
-        if (ok) {
-          umma::commit(empty + 8 * v_slot);
-          if (more) {
-            umma::commit(empty + 8 * k_slot);
-            next_slot();
-          }
+        end_turn();
+        release(2 * j + 1, j < mine);
+        if (more) {
+          release(2 * j + 2, j + 1 < mine);
         }
       }
       if (!ok) {
@@ -1003,12 +1004,12 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
+  if (*fail_flag != 0u && (warp == 8 || warp == 11) && lane == 0) {
+    umma::commit(drain);  // MMAs still in flight, if any
+  }
+  __syncwarp();
   if (warp == 8) {
     if (*fail_flag != 0u) {
-      if (lane == 0) {
-        umma::commit(drain);  // MMAs still in flight, if any
-      }
-      __syncwarp();
       (void)wait_for(drain, 0);
     }
     umma::tmem_dealloc(tmem, 512);
