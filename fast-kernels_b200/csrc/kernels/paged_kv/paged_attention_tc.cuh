@@ -88,6 +88,8 @@ struct TcLayout {
   static constexpr int kRowPower = kTileLogs + (kQuant ? kFactorRing * 16 : 0);     // [256]
   static constexpr int kBarriers = kRowPower + (kQuant ? 1024 : 0);
   static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
+  // results are staged over the operands
+  static_assert(2 * kTileRows * (D + 4) * 4 <= kRing + kSlots * kOperandBytes, "rows of results fit the operands' memory");
 };
 
 // Bounded wait. The plain test comes first: most waits of the issuer and the copies are over when they
@@ -122,6 +124,14 @@ __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
       "l"(map), "r"(x), "r"(y), "r"(bar)
       : "memory");
+}
+// Shared memory -> global, both 16-byte aligned, `bytes` a multiple of 16.
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+// This thread's bulk stores are complete.
+__device__ __forceinline__ void bulk_store_wait() {
+  asm volatile("cp.async.bulk.commit_group;\ncp.async.bulk.wait_group 0;" ::: "memory");
 }
 // Operand descriptors: 128-byte swizzle (bits 61-63 = 2), version 1 (bit 46), offsets in 16-byte units.
 // Rows are the M or N dimension (K contiguous): groups of 8 rows are 1024 bytes apart.
@@ -626,18 +636,22 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       }
     }
     // ---- results --------------------------------------------------------------------------------
-    const bool write_row = fits && r < rows && vec.x >= 0 && vec.x < p.num_rows;
+    // Every thread lays its row out in shared memory (once both row tiles are done with the operands there)
+    // and a bulk copy takes it away: stores straight from a thread per row touch 32 lines an instruction,
+    // 9000 clocks for 256 rows of partial results.
     if (tiles[x] > 0 && ok && !wait_for(o_final + 8 * x, 0)) {
       give_up();
       ok = false;
     }
-    if (ok && x * kTileRows < rows && fits) {
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (ok && x * kTileRows < rows && fits && *fail_flag == 0u) {
       umma::fence_after_sync();
       const bool direct = item.partial < 0;
-      const bool slot_fits = direct || (item.partial < vec.w && vec.z >= 0 && vec.z + item.partial < p.num_partials);
+      const bool write_row = r < rows && vec.x >= 0 && vec.x < p.num_rows &&
+                             (direct || (item.partial < vec.w && vec.z >= 0 && vec.z + item.partial < p.num_partials));
       const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-      uint16_t* out = p.output + (static_cast<size_t>(vec.x) * p.num_q_heads + my_head) * D;
-      float* part = p.partials + (static_cast<size_t>(vec.z + item.partial) * p.num_q_heads + my_head) * (D + 4);
+      constexpr uint32_t kRowBytes = (D + 4) * 4;  // 16 bytes off a multiple of 128: lanes take turns at the banks
+      const uint32_t staged = base + r * kRowBytes;
 #pragma unroll
       for (int c = 0; c < D; c += 32) {
         uint32_t o[32];
@@ -649,28 +663,36 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           tile::ld32(o_tmem + c, o);
           tile::wait_ld32(o);
         }
-        if (write_row && slot_fits) {
-          if (direct) {
+        if (direct) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              uint4 w;
-              w.x = pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-              w.y = pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-              w.z = pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-              w.w = pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-              *reinterpret_cast<uint4*>(out + c + i) = w;
-            }
-          } else {
+          for (int i = 0; i < 32; i += 8) {
+            uint4 w;
+            w.x = pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+            w.y = pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+            w.z = pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+            w.w = pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+            sts128(staged + (c + i) * 2, w);
+          }
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              *reinterpret_cast<uint4*>(part + c + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-            }
+          for (int i = 0; i < 32; i += 4) {
+            sts128(staged + (c + i) * 4, make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]));
           }
         }
       }
-      if (write_row && slot_fits && !direct) {
-        *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+      if (!direct) {
+        sts128(staged + D * 4, make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
       }
+      proxy_fence_async();
+      if (write_row) {
+        if (direct) {
+          bulk_store(p.output + (static_cast<size_t>(vec.x) * p.num_q_heads + my_head) * D, staged, D * 2);
+        } else {
+          bulk_store(p.partials + (static_cast<size_t>(vec.z + item.partial) * p.num_q_heads + my_head) * (D + 4), staged,
+                     kRowBytes);
+        }
+      }
+      bulk_store_wait();
     }
   } else {
     tile::registers_down<L::kOtherRegisters>();

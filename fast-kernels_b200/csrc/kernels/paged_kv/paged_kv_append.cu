@@ -52,7 +52,12 @@ void fill_rope_table(RopeTable* table, int head_dim, float theta) {
   thread_local float kept_theta = 0.0f;
   if (kept_dim != head_dim || kept_theta != theta) {
     for (int i = 0; i < head_dim / 2; ++i) {
-      kept.turns[i] = std::pow(static_cast<double>(theta), -2.0 * i / head_dim) / 6.283185307179586476925286766559;
+      // long double: 64 bits of mantissa, so that far positions lose nothing (a theta below 1 turns pairs by
+      // more than a turn per position; the whole turns do not matter)
+      const long double turns = std::pow(static_cast<long double>(theta), -2.0L * i / head_dim) / 6.283185307179586476925286766559L;
+      const long double fraction = turns - std::floor(turns);
+      const long double scaled = std::round(fraction * 18446744073709551616.0L);
+      kept.turns[i] = scaled >= 18446744073709551616.0L ? 0 : static_cast<uint64_t>(scaled);
     }
     kept_dim = head_dim;
     kept_theta = theta;

@@ -17,17 +17,17 @@ constexpr int kKvInt8 = FK_PAGED_KV_INT8;
 constexpr int kScaleBlock = 64;  // dimensions that share a scale
 constexpr int kMaxPairs = 64;
 
-// Turns per position of every rotary pair: theta^(-2i/d) / (2 pi), in fp64. A position times this has
-// the whole turns taken off before anything is rounded to fp32, so the angle's error does not grow
-// with the position (an fp32 product is off by up to 2^-8 radians at position 131072).
+// Turns per position of every rotary pair, theta^(-2i/d) / (2 pi), in units of 2^-64: a position times
+// this, modulo 2^64, is the angle with the whole turns taken off, off by at most 2^-34 turns at any
+// 31-bit position (an fp32 product is off by up to 2^-8 radians at position 131072).
 struct RopeTable {
-  double turns[kMaxPairs];
+  uint64_t turns[kMaxPairs];
 };
 void fill_rope_table(RopeTable* table, int head_dim, float theta);
 
-__device__ __forceinline__ float2 rope_cos_sin(double turns_per_position, int position) {
-  const double turns = turns_per_position * static_cast<double>(position);
-  const float half_turns = 2.0f * static_cast<float>(turns - rint(turns));
+__device__ __forceinline__ float2 rope_cos_sin(uint64_t turns_per_position, int position) {
+  const uint64_t turns = turns_per_position * static_cast<uint32_t>(position);
+  const float half_turns = static_cast<float>(static_cast<int32_t>(turns >> 32)) * 0x1p-31f;  // in [-1, 1]
   float sn, cs;
   sincospif(half_turns, &sn, &cs);
   return make_float2(cs, sn);

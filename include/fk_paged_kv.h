@@ -46,7 +46,7 @@ extern "C" {
  * segment that does not fit the page, the pool or the rows is left out.
  *
  * With rotate_keys != 0 dimensions 2i and 2i + 1 of a key are turned by position * theta^(-2i/head_dim)
- * (the angle's fraction of a turn is taken in fp64, the turn is fp32).
+ * (the angle's fraction of a turn is taken in 64-bit fixed point, the turn is fp32).
  *   bf16 pages: the turned key is rounded once; values are copied.
  *   8-bit pages, L = 127 (int8) or 448 (e4m3): a value is stored as round(v / s) with
  *   s = max(max|v| / L, 1e-6) over the token's 64-dim block. A key block's scale belongs to the page:
