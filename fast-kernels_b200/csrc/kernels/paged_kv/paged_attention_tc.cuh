@@ -24,7 +24,8 @@
 //
 // Roles (warps): 0-3 and 4-7 softmax of the two row tiles (they also turn and store the queries, and
 // write the results), 8 and 11 issue the two tiles' MMAs, 9 the copies, 10 clears the value rows behind the end (a
-// probability of 0 times whatever a page holds there would not be 0). 8-bit pages: 12-15 convert.
+// probability of 0 times whatever a page holds there would not be 0). 8-bit pages: 12-15 convert (where
+// there is only one row tile, keys; the other tile's softmax warps convert the values).
 // Every wait is bounded.
 //
 // Operands in shared memory are rows of 128 bytes (64 16-bit elements) under the 128-byte swizzle; a
@@ -86,7 +87,8 @@ struct TcLayout {
   static constexpr int kRatios = kRawKeyScales + kRawSlots * 64;                    // [8 pages + 128 tokens][2]
   static constexpr int kTileLogs = kRatios + (kQuant ? 64 + 1024 : 0);              // [ring][4 warps]
   static constexpr int kRowPower = kTileLogs + (kQuant ? kFactorRing * 16 : 0);     // [256]
-  static constexpr int kBarriers = kRowPower + (kQuant ? 1024 : 0);
+  static constexpr int kTurns = kRowPower + (kQuant ? 1024 : 0);                    // [64]
+  static constexpr int kBarriers = kTurns + 512;
   static constexpr int kBytes = kBarriers + 512 + 1024;            // and the alignment's slack
   // results are staged over the operands
   static_assert(2 * kTileRows * (D + 4) * 4 <= kRing + kSlots * kOperandBytes, "rows of results fit the operands' memory");
@@ -291,9 +293,12 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     }
     mbar_init_fence();
   }
+  uint64_t* turns = reinterpret_cast<uint64_t*>(smem + L::kTurns);
   if (warp == 8) {
     umma::tmem_alloc(bars, 512);
     umma::tmem_relinquish();
+  } else if (warp == 10) {
+    share_rope_table(p.rope, turns, D / 2, lane);
   }
   umma::fence_before_sync();
   __syncthreads();
@@ -333,6 +338,120 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   auto give_up = [&]() {
     *fail_flag = 1u;
     atomicExch(p.status, kStatusWaitTimeout);
+  };
+
+  // ---- 8-bit tiles to 16 bits: 128 threads, tiles `begin`, `begin` + `stride`, ... of keys 2 j and values 2 j + 1
+  auto convert = [&](int t, int begin, int stride, auto barrier) {
+      constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
+      constexpr int kPasses = kTileTokens / kRowsPerPass;
+      // A thread's rows are first + pass * kRowsPerPass, a batch at a time: all loads, all arithmetic, all
+      // stores. (The loads and stores are volatile: in the order of one row after the other every row
+      // waits for the one before, 230 clocks each.)
+      constexpr int kBatch = 4;
+      uint32_t* key_ratios = reinterpret_cast<uint32_t*>(smem + L::kRatios);  // [8 pages][2 blocks]
+      uint32_t* value_ratios = key_ratios + 16;                               // [128 rows][2 blocks]
+      const int page_shift = p.page_size == 16 ? 4 : 5;
+      const int chunk = t % kChunks;
+      const int block = chunk / 8;
+      const int first = t / kChunks;
+      bool ok = true;
+      for (int i = begin; ok && i < 2 * count; i += stride) {
+        const int raw_slot = i % (QUANT ? L::kRawSlots : 1);
+        const int slot = i % L::kSlots;
+        const int raw_use = i / (QUANT ? L::kRawSlots : 1);
+        const int use = i / L::kSlots;
+        const int j = i >> 1;
+        const bool keys = (i & 1) == 0;
+        // In this order: with every other tile the group does not see a raw slot's every phase, but tile
+        // i - kSlots being released says that the copies before this one have landed, so that the parity
+        // can only mean this one.
+        static_assert(!QUANT || L::kRawSlots >= L::kSlots, "a raw slot's previous tile is released with the operand slot's");
+        ok = (use == 0 || wait_for(empty + 8 * slot, (use - 1) & 1)) && wait_for(raw_full + 8 * raw_slot, raw_use & 1);
+        if (!ok) {
+          break;
+        }
+        const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
+        const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
+        const int valid = min(kTileTokens, loaded - j * kTileTokens);
+        const uint32_t* ratios = keys ? key_ratios : value_ratios;
+        if (keys) {
+          if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
+            const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + t * 8);
+            const float larger = fmaxf(s.x, s.y);
+            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + t] = larger;
+            if constexpr (kBlocks == 2) {
+              key_ratios[2 * t] = scale_ratio(s.x, larger);
+              key_ratios[2 * t + 1] = scale_ratio(s.y, larger);
+            }
+          }
+        } else {
+          // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
+          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes) + t * kBlocks;
+          float larger = scales[0];
+          if constexpr (kBlocks == 2) {
+            larger = fmaxf(larger, scales[1]);
+            value_ratios[2 * t] = scale_ratio(scales[0], larger);
+            value_ratios[2 * t + 1] = scale_ratio(scales[1], larger);
+          }
+          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
+          factors[0] = t < valid ? larger : 0.0f;
+          // (a scale of 0 must not leave a tile without a finite heaviest weight)
+          const float log = t < valid ? __log2f(fmaxf(larger, 1e-30f)) : -INFINITY;
+          factors[kFactorRing * kTileTokens] = log;
+          float most = log;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          }
+          if (lane == 0) {
+            reinterpret_cast<float*>(smem + L::kTileLogs)[(j % kFactorRing) * 4 + (warp & 3)] = most;
+          }
+        }
+        if constexpr (kBlocks == 2) {
+          asm volatile("bar.sync %0, 128;" ::"n"(decltype(barrier)::value) : "memory");  // the ratios, by the rows' other threads
+        }
+#pragma unroll
+        for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
+          uint2 w[kBatch];
+          uint32_t ratio[kBatch];
+          uint4 out[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = first + (pass0 + b) * kRowsPerPass;
+            w[b] = lds64(from + row * D + chunk * 8);
+            ratio[b] = kBlocks == 2 ? ratios[(keys ? row >> page_shift : row) * 2 + block] : 0u;
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = first + (pass0 + b) * kRowsPerPass;
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out[b].x, out[b].y);
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out[b].z, out[b].w);
+            if constexpr (kBlocks == 2) {
+              out[b].x = mul_half2(out[b].x, ratio[b]);
+              out[b].y = mul_half2(out[b].y, ratio[b]);
+              out[b].z = mul_half2(out[b].z, ratio[b]);
+              out[b].w = mul_half2(out[b].w, ratio[b]);
+            }
+            // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
+            if (row >= valid) {
+              out[b] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            sts128(to + operand_chunk(first + (pass0 + b) * kRowsPerPass, chunk), out[b]);
+          }
+        }
+        proxy_fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          umma::mbar_arrive(full + 8 * slot);
+          umma::mbar_arrive(raw_empty + 8 * raw_slot);
+        }
+      }
+      if (!ok) {
+        give_up();
+      }
   };
 
   if (warp < 8) {
@@ -376,7 +495,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           if (h0 == 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float2 turn = rope_cos_sin(p.rope.turns[chunk * 4 + i], position);
+              const float2 turn = rope_cos_sin(turns[chunk * 4 + i], position);
               cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
             }
           }
@@ -439,6 +558,11 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         umma::mbar_arrive(q_ready);
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");  // row_power is read by other warps than its writers
+    }
+    if constexpr (QUANT) {
+      if (x == 1 && tiles[1] == 0 && count > 0) {  // no rows of its own: the values are converted here
+        convert(tid - 128, 1, 2, std::integral_constant<int, 3>{});
+      }
     }
     // ---- softmax --------------------------------------------------------------------------------
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -904,120 +1028,8 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         give_up();
       }
     } else if (QUANT && warp >= 12 && count > 0) {
-      // ---- 8-bit tiles to 16 bits ---------------------------------------------------------------
-      constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
-      constexpr int kPasses = kTileTokens / kRowsPerPass;
-      // A thread's rows are first + pass * kRowsPerPass, a batch at a time: all loads, all arithmetic, all
-      // stores. (The loads and stores are volatile: in the order of one row after the other every row
-      // waits for the one before, 230 clocks each.)
-      constexpr int kBatch = 4;
-      uint32_t* key_ratios = reinterpret_cast<uint32_t*>(smem + L::kRatios);  // [8 pages][2 blocks]
-      uint32_t* value_ratios = key_ratios + 16;                               // [128 rows][2 blocks]
-      const int t = tid - 384;
-      const int page_shift = p.page_size == 16 ? 4 : 5;
-      const int chunk = t % kChunks;
-      const int block = chunk / 8;
-      const int first = t / kChunks;
-      int raw_slot = 0, slot = 0;
-      uint32_t raw_uses = 0, uses = 0;
-      bool ok = true;
-      for (int i = 0; ok && i < 2 * count; ++i) {
-        const int j = i >> 1;
-        const bool keys = (i & 1) == 0;
-        ok = wait_for(raw_full + 8 * raw_slot, raw_uses & 1) &&
-             (uses == 0 || wait_for(empty + 8 * slot, (uses - 1) & 1));
-        if (!ok) {
-          break;
-        }
-        const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
-        const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
-        const int valid = min(kTileTokens, loaded - j * kTileTokens);
-        const uint32_t* ratios = keys ? key_ratios : value_ratios;
-        if (keys) {
-          if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
-            const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + t * 8);
-            const float larger = fmaxf(s.x, s.y);
-            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + t] = larger;
-            if constexpr (kBlocks == 2) {
-              key_ratios[2 * t] = scale_ratio(s.x, larger);
-              key_ratios[2 * t + 1] = scale_ratio(s.y, larger);
-            }
-          }
-        } else {
-          // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
-          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes) + t * kBlocks;
-          float larger = scales[0];
-          if constexpr (kBlocks == 2) {
-            larger = fmaxf(larger, scales[1]);
-            value_ratios[2 * t] = scale_ratio(scales[0], larger);
-            value_ratios[2 * t + 1] = scale_ratio(scales[1], larger);
-          }
-          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
-          factors[0] = t < valid ? larger : 0.0f;
-          // (a scale of 0 must not leave a tile without a finite heaviest weight)
-          const float log = t < valid ? __log2f(fmaxf(larger, 1e-30f)) : -INFINITY;
-          factors[kFactorRing * kTileTokens] = log;
-          float most = log;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          }
-          if (lane == 0) {
-            reinterpret_cast<float*>(smem + L::kTileLogs)[(j % kFactorRing) * 4 + (warp & 3)] = most;
-          }
-        }
-        if constexpr (kBlocks == 2) {
-          asm volatile("bar.sync 2, 128;" ::: "memory");  // the ratios, by the rows' other threads
-        }
-#pragma unroll
-        for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
-          uint2 w[kBatch];
-          uint32_t ratio[kBatch];
-          uint4 out[kBatch];
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            const int row = first + (pass0 + b) * kRowsPerPass;
-            w[b] = lds64(from + row * D + chunk * 8);
-            ratio[b] = kBlocks == 2 ? ratios[(keys ? row >> page_shift : row) * 2 + block] : 0u;
-          }
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            const int row = first + (pass0 + b) * kRowsPerPass;
-            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out[b].x, out[b].y);
-            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out[b].z, out[b].w);
-            if constexpr (kBlocks == 2) {
-              out[b].x = mul_half2(out[b].x, ratio[b]);
-              out[b].y = mul_half2(out[b].y, ratio[b]);
-              out[b].z = mul_half2(out[b].z, ratio[b]);
-              out[b].w = mul_half2(out[b].w, ratio[b]);
-            }
-            // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
-            if (row >= valid) {
-              out[b] = make_uint4(0u, 0u, 0u, 0u);
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            sts128(to + operand_chunk(first + (pass0 + b) * kRowsPerPass, chunk), out[b]);
-          }
-        }
-        proxy_fence_async();
-        __syncwarp();
-        if (lane == 0) {
-          umma::mbar_arrive(full + 8 * slot);
-          umma::mbar_arrive(raw_empty + 8 * raw_slot);
-        }
-        if (++slot == L::kSlots) {
-          slot = 0;
-          ++uses;
-        }
-        if (++raw_slot == L::kRawSlots) {
-          raw_slot = 0;
-          ++raw_uses;
-        }
-      }
-      if (!ok) {
-        give_up();
+      if constexpr (QUANT) {
+        convert(tid - 384, 0, tiles[1] > 0 ? 1 : 2, std::integral_constant<int, 2>{});
       }
     }
   }

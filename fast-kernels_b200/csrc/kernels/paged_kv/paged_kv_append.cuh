@@ -111,8 +111,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_kv_append_kernel(cons
   constexpr int kSteps = PS / kRowsPerStep;
   constexpr int kBlocks = D / kScaleBlock;
   __shared__ float2 table[ROT ? PS * (D / 2) : 1];  // [token][pair]: cos, sin
+  __shared__ uint64_t turns[ROT ? D / 2 : 1];
 
   fk_w4a16::pdl_launch_dependents();
+  if constexpr (ROT) {
+    if (threadIdx.x < 32) {
+      share_rope_table(p.rope, turns, D / 2, threadIdx.x);
+    }
+    __syncthreads();
+  }
   fk_w4a16::pdl_wait_for_prerequisites();
   const int4 segment = p.segments[blockIdx.x];
   const int page = segment.x;
@@ -154,7 +161,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_kv_append_kernel(cons
     }
     if (ROT && head0 == 0) {
       for (int i = threadIdx.x; i < count * (D / 2); i += kAppendWarps * 32) {
-        table[i] = rope_cos_sin(p.rope.turns[i % (D / 2)], segment.w + i / (D / 2));
+        table[i] = rope_cos_sin(turns[i % (D / 2)], segment.w + i / (D / 2));
       }
       __syncthreads();
     }

@@ -25,6 +25,17 @@ struct RopeTable {
 };
 void fill_rope_table(RopeTable* table, int head_dim, float theta);
 
+// The table from the kernel's parameters to shared memory, by one warp: a parameter indexed by the lane is
+// read one lane at a time (3000 clocks for the four pairs of 256 threads).
+__device__ __forceinline__ void share_rope_table(const RopeTable& table, uint64_t* shared, int pairs, int lane) {
+#pragma unroll 8
+  for (int i = 0; i < pairs; ++i) {
+    const uint64_t turns = table.turns[i];
+    if (lane == (i & 31)) {
+      shared[i] = turns;
+    }
+  }
+}
 __device__ __forceinline__ float2 rope_cos_sin(uint64_t turns_per_position, int position) {
   const uint64_t turns = turns_per_position * static_cast<uint32_t>(position);
   const float half_turns = static_cast<float>(static_cast<int32_t>(turns >> 32)) * 0x1p-31f;  // in [-1, 1]
