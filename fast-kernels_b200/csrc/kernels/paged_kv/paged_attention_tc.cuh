@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           if (h0 == 0) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const float2 turn = rope_cos_sin(turns[chunk * 4 + i], position);
+              const float2 turn = rope_cos_sin_quick(turns[chunk * 4 + i], position);
               cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
             }
           }

@@ -44,6 +44,13 @@ __device__ __forceinline__ float2 rope_cos_sin(uint64_t turns_per_position, int 
   return make_float2(cs, sn);
 }
 
+// The same, off by up to 2^-20.5: for a query that is rounded to 16 bits behind it.
+__device__ __forceinline__ float2 rope_cos_sin_quick(uint64_t turns_per_position, int position) {
+  const uint64_t turns = turns_per_position * static_cast<uint32_t>(position);
+  const float angle = static_cast<float>(static_cast<int32_t>(turns >> 32)) * (0x1p-32f * 6.2831853071795865f);
+  return make_float2(__cosf(angle), __sinf(angle));
+}
+
 __device__ __forceinline__ float bf16_low(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf16_high(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
