@@ -961,6 +961,60 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
   const int priors = split == 0 ? prior_rows.y : 0;
   const size_t prior_step = static_cast<size_t>(p.num_q_heads) * ROW;
   float* my_partial = p.partials + (static_cast<size_t>(task) * S + split) * (GT * ROW);
+  // The prior rows join the block's own result first, kMaxSplits at a time, as one more warp's: every
+  // thread that adds values has all its rows in flight, and their weights come from shared memory.
+  for (int j0 = 0; j0 < priors; j0 += kMaxSplits) {
+    const int here = min(kMaxSplits, priors - j0);
+    const float* rows = p.prior + (static_cast<size_t>(prior_rows.x + j0) * p.num_q_heads + first_q_head) * ROW;
+    for (int idx = tid; idx < tile_heads * here; idx += threads) {
+      const int h = idx / here;
+      const int j = idx - h * here;
+      const float2 ml = __ldcg(reinterpret_cast<const float2*>(rows + j * prior_step + h * ROW + D));
+      split_m[h * kMaxSplits + j] = ml.x;
+      split_l[h * kMaxSplits + j] = ml.y;
+    }
+    __syncthreads();
+    if (tid < tile_heads) {  // into warp 0's maximum and denominator; its values keep `keep`
+      const float m_old = merge_m[tid];
+      float m_all = m_old;
+      for (int j = 0; j < here; ++j) {
+        m_all = fmaxf(m_all, split_m[tid * kMaxSplits + j]);
+      }
+      const float m_ref = m_all == -INFINITY ? 0.0f : m_all;
+      const float keep = exp2f(m_old - m_ref);
+      float l_all = keep * merge_l[tid];
+      for (int j = 0; j < here; ++j) {
+        const float weight = exp2f(split_m[tid * kMaxSplits + j] - m_ref);
+        l_all += weight * split_l[tid * kMaxSplits + j];
+        split_m[tid * kMaxSplits + j] = weight;
+      }
+      merge_m[tid] = m_all;
+      merge_l[tid] = l_all;
+      block_result[tid * ROW] = keep;
+    }
+    __syncthreads();
+    for (int idx = tid; idx < tile_heads * (D / 4); idx += threads) {
+      const int h = idx / (D / 4);
+      const int d = (idx - h * (D / 4)) * 4;
+      float* mine = &merge_acc[h * D + d];
+      const float keep = block_result[h * ROW];
+      float4 sum = make_float4(keep * mine[0], keep * mine[1], keep * mine[2], keep * mine[3]);
+#pragma unroll 8
+      for (int j = 0; j < here; ++j) {
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(rows + j * prior_step + h * ROW + d));
+        const float weight = split_m[h * kMaxSplits + j];
+        sum.x = fmaf(weight, v.x, sum.x);
+        sum.y = fmaf(weight, v.y, sum.y);
+        sum.z = fmaf(weight, v.z, sum.z);
+        sum.w = fmaf(weight, v.w, sum.w);
+      }
+      mine[0] = sum.x;
+      mine[1] = sum.y;
+      mine[2] = sum.z;
+      mine[3] = sum.w;
+    }
+    __syncthreads();
+  }
   for (int idx = tid; idx < tile_heads * D; idx += threads) {
     const int h = idx / D;
     const int d = idx - h * D;
@@ -968,27 +1022,12 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
     for (int w = 0; w < warps; ++w) {
       m_all = fmaxf(m_all, merge_m[w * GT + h]);
     }
-    const float* prior_row = nullptr;
-    if (priors > 0) {
-      prior_row = p.prior + (static_cast<size_t>(prior_rows.x) * p.num_q_heads + first_q_head + h) * ROW;
-#pragma unroll 8
-      for (int j = 0; j < priors; ++j) {
-        m_all = fmaxf(m_all, __ldcg(prior_row + j * prior_step + D));
-      }
-    }
     const float m_ref = m_all == -INFINITY ? 0.0f : m_all;
     float l_all = 0.0f, a_all = 0.0f;
     for (int w = 0; w < warps; ++w) {
       const float weight = exp2f(merge_m[w * GT + h] - m_ref);
       l_all += weight * merge_l[w * GT + h];
       a_all += weight * merge_acc[(w * GT + h) * D + d];
-    }
-#pragma unroll 8
-    for (int j = 0; j < priors; ++j) {
-      const float2 ml = __ldcg(reinterpret_cast<const float2*>(prior_row + j * prior_step + D));
-      const float weight = exp2f(ml.x - m_ref);
-      l_all += weight * ml.y;
-      a_all += weight * __ldcg(prior_row + j * prior_step + d);
     }
     if (S == 1) {
       const float y = l_all == 0.0f ? 0.0f : a_all / l_all;
