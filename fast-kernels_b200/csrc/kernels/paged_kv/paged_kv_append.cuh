@@ -94,6 +94,13 @@ __device__ __forceinline__ float largest8(const float (&x)[8]) {
   }
   return m;
 }
+// x / s, rounded as a division rounds it, from r = 1 / s rounded: one Newton step on the quotient (Markstein,
+// "Computation of elementary functions on the IBM RISC System/6000 processor", 1990). Sixteen divisions
+// a step were most of the kernel's instructions.
+__device__ __forceinline__ float quotient(float x, float s, float r) {
+  const float q = x * r;
+  return fmaf(fmaf(-q, s, x), r, q);
+}
 // Maximum over the eight lanes that hold one token's 64-dim block.
 __device__ __forceinline__ float largest_of_block(float m) {
 #pragma unroll
@@ -208,6 +215,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_kv_append_kernel(cons
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
       }
       const float scale = fmaxf(held, fmaxf(largest / Q::kLimit, 1e-6f));
+      const float key_inverse = __frcp_rn(scale);
       if (scale > held) {  // (the same on all lanes of the block)
         // what the page holds already, brought to the larger scale
         for (int t = row; t < slot; t += kRowsPerStep) {
@@ -233,6 +241,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_kv_append_kernel(cons
         float x[8], y[8];
         unpack8(v[s], y);  // (zeros past the segment: every lane takes part in the shuffles)
         const float value_scale = fmaxf(largest_of_block(largest8(y)) / Q::kLimit, 1e-6f);
+        const float value_inverse = __frcp_rn(value_scale);
         if (t < count) {
           unpack8(k[s], x);
           if constexpr (ROT) {
@@ -240,8 +249,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32) paged_kv_append_kernel(cons
           }
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
-            x[i] = x[i] / scale;
-            y[i] = y[i] / value_scale;
+            x[i] = quotient(x[i], scale, key_inverse);
+            y[i] = quotient(y[i], value_scale, value_inverse);
           }
           const size_t at = first + static_cast<size_t>(s) * kRowsPerStep * D;
           *reinterpret_cast<uint2*>(p.key_pages + at) =

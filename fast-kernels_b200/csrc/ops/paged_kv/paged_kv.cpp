@@ -106,8 +106,8 @@ void shared_prefix_decode_forward(
     std::uintptr_t partials_ptr, int batch, int num_page_ids, int num_items, int num_partials, int num_runs,
     int max_tail_pages, int num_pages, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int kv_format,
     float softmax_scale, float rope_theta, std::uintptr_t stream_ptr) {
-  if (num_items <= 0 || num_partials <= 0) {
-    throw std::invalid_argument("shared_prefix_decode needs items and partial results");
+  if (num_items < 0 || (num_items > 0) != (num_partials > 0)) {
+    throw std::invalid_argument("shared_prefix_decode: items and partial results come together");
   }
   fk_page_decode_args tail{};
   tail.query = as<const void>(query_ptr);
@@ -172,9 +172,14 @@ void shared_prefix_decode_forward(
   args.softmax_scale = softmax_scale;
   args.rope_theta = rope_theta;
   args.stream = tail.stream;
-  raise_if_failed(fk_paged_kv_attention(&args));
-  fk_page_decode_prior prior{as<const float>(partials_ptr), as<const int32_t>(of_request_ptr)};
-  const int code = fk_page_decode_forward_merged(&tail, &prior);
+  int code = FK_PAGE_DECODE_OK;
+  if (num_items > 0) {
+    raise_if_failed(fk_paged_kv_attention(&args));
+    fk_page_decode_prior prior{as<const float>(partials_ptr), as<const int32_t>(of_request_ptr)};
+    code = fk_page_decode_forward_merged(&tail, &prior);
+  } else {
+    code = fk_page_decode_forward(&tail);
+  }
   if (code == FK_PAGE_DECODE_ERR_INVALID_ARGUMENT) {
     throw std::invalid_argument(fk_page_decode_last_error());
   }

@@ -40,9 +40,9 @@ from fast_kernels.ops.clustered_page_decode import (
 from fast_kernels.ops.prefix_union_decode import _shared_page_bytes
 
 _PLANS: OrderedDict = OrderedDict()
-# Bytes that a plan has to save before it shares: what the kernels behind a shared run cost more than
-# the decode kernel alone, times the HBM rate.
-DEFAULT_MIN_SAVED_BYTES = 32 << 20
+# Bytes that a plan has to save before it shares. Measured with 8 kv heads of 128, us with sharing / without: bf16, 62 MB
+# saved 24.5 / 20.5, 124 MB 24.6 / 26.7, 248 MB 26.7 / 41.1; int8, 32 MB 28.6 / 22.6, 64 MB 28.7 / 30.9, 128 MB 32.8 / 49.4.
+DEFAULT_MIN_SAVED_BYTES = 64 << 20
 # Shared runs shorter than this stay with the requests (or with longer runs further down).
 MIN_RUN_TOKENS = 128
 
@@ -240,18 +240,22 @@ def shared_prefix_decode(
         _paged.check_output(output, shape=shape, device=device)
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(plan.head_dim)
     with _paged.current(device):
-        if not plan.runs:
-            return clustered_page_decode(query, cache, plan=plan.tail_plan, output=output, softmax_scale=scale,
-                                         rope_theta=rope_theta)
         stream = _paged.current_stream(device)
         tables = plan.device_tables(device, stream)
-        partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
+        # (the plain decode may split long requests through scratch that belongs to the stream, which graphs that
+        # were captured on it would share; a captured call does without)
+        if not plan.runs and not torch.cuda.is_current_stream_capturing():
+            return clustered_page_decode(query, cache, plan=plan.tail_plan, output=output, softmax_scale=scale,
+                                         rope_theta=rope_theta)
+        partials = None
+        if plan.runs:
+            partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
         tail = plan.tail_plan
         native.shared_prefix_decode_forward(
             query.data_ptr(), cache.key_pages.data_ptr(), cache.value_pages.data_ptr(), _paged.address(cache.key_scales),
             _paged.address(cache.value_scales), tables["page_ids"], tables["vectors"], tables["items"], tables["of_request"],
             tables["run_base_pages"], tables["run_page_counts"], tables["run_logical_starts"], tables["run_last_page_lens"],
-            tables["request_run_offsets"], tables["seq_lens"], output.data_ptr(), partials.data_ptr(), plan.batch,
+            tables["request_run_offsets"], tables["seq_lens"], output.data_ptr(), _paged.address(partials), plan.batch,
             plan.page_ids_cpu.shape[0], plan.num_items, plan.num_partials, tail.num_runs, tail.max_pages,
             cache.key_pages.shape[0], plan.num_q_heads, plan.num_kv_heads, plan.head_dim, plan.page_size,
             _layout_id(plan.kv_layout), float(scale), float(rope_theta), stream)

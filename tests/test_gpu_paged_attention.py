@@ -375,6 +375,25 @@ def test_shared_same_bits_every_time_on_streams_and_in_graphs() -> None:
     _status_ok()
 
 
+def test_without_sharing_a_captured_call_needs_no_call_before_it() -> None:
+    """Long requests on a stream that has made no call yet: the plain decode would want scratch of the stream's."""
+    counts = [200, 3]
+    table, pages = fragmented_table(counts, 1)
+    cache = random_cache(layout="bf16_kv", pages=pages, heads=2, page_size=16, dim=64, table=table, lens=[3199, 40], theta=THETA, seed=2)
+    query = _query(2, 8, 64, 3)
+    plan = _shared_plan(cache, 8)
+    assert plan.runs == []
+    plan.device_tables(query.device, torch.cuda.current_stream().cuda_stream)
+    output = torch.empty_like(query)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        ops.shared_prefix_decode(query, cache, plan=plan, output=output)
+    graph.replay()
+    torch.cuda.synchronize()
+    _assert_rows(output, cache, query, [(0, 3198), (1, 39)], default_scale(64))
+    _status_ok()
+
+
 def test_shared_refusals() -> None:
     cache = _shared("bf16_kv")
     query = _query(10, 8, 64, 5)
