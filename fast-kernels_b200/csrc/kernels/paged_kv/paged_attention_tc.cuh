@@ -19,21 +19,29 @@
 // are: their commit follows the previous tile's second product.
 //
 // The exponentials are what the softmax warps are bound by (16 a clock and SM: 2048 clocks per token tile
-// and 256 rows, the two products take as long). With bf16 pages a quarter of them, in tiles without a
-// mask, is a polynomial on the FMA pipe.
+// and 256 rows, the two products take as long).
 //
 // Roles (warps): 0-3 and 4-7 softmax of the two row tiles (they also turn and store the queries, and
-// write the results), 8 and 11 issue the two tiles' MMAs, 9 the copies, 10 clears the value rows behind the end (a
-// probability of 0 times whatever a page holds there would not be 0). 8-bit pages: 12-15 convert (where
-// there is only one row tile, keys; the other tile's softmax warps convert the values).
-// Every wait is bounded.
+// write the results), 8 and 11 issue the two tiles' MMAs, 9 the copies, 10 clears the value
+// rows behind the end (a probability of 0 times whatever a page holds there would not be 0). 8-bit pages:
+// 12-15 convert. Every wait is bounded.
 //
 // Operands in shared memory are rows of 128 bytes (64 16-bit elements) under the 128-byte swizzle; a
 // tile of 128-dimensional rows is two such halves. bf16 pages are copied there by TMA, one box of
-// page_size rows per page and half. 8-bit pages are copied as they are and converted by four warps:
-// keys to fp16, exact for the 64-dim block with the page's larger scale, the other block times the
-// ratio of the two scales; values to bf16 likewise per token. The larger scales stay fp32: the page's
-// goes on the logits, the token's on the probability before it is rounded.
+// page_size rows per page and half. 8-bit pages are copied as they are and converted by four warps to
+// fp16, exactly for the 64-dim block with the page's (keys) or token's (values) larger scale, the other
+// block times the ratio of the two scales. The larger scales stay fp32: the page's goes on the logits,
+// the token's on the probability before it is rounded. (Values in bf16 with bf16 probabilities took five
+// times the conversion's instructions, and their two roundings made the error 1.5 times the output's own.)
+//
+// What it measures: 8192 tokens, 32 heads over 8 of 128, bf16, causal: 594 us, 925 TFLOP/s, 57 % of the
+// measured bf16 peak: a token tile takes 3450 clocks where the products need 2050. 512 tokens behind 32768
+// in fp8 pages, 32 heads over 4: 474 us, 584 TFLOP/s: bound by the conversion (3800 clocks a tile, in the
+// issue slots of the softmax warps) and the chain behind it.
+// Tried and slower: steps of 64 tokens with two buffers of logits per row tile (N = 64 costs the tensor
+// core as much as N = 128 when both operands come from shared memory: 748 us), four more converting warps
+// (fewer registers for the softmax: 602 us for 477), a quarter or half of the exponentials as polynomials
+// on the FMA pipe (613 and 640 us for 594).
 #pragma once
 
 #include <cuda.h>
@@ -201,27 +209,6 @@ __device__ __forceinline__ float largest_of(const uint32_t* r) {
   return max3(a, b, max3(a, __uint_as_float(r[N - 2]), __uint_as_float(r[N - 1])));
 }
 
-// 2^x for two x <= 8 on the FMA pipe: x = i + f, |f| <= 1/2, a polynomial of degree 4 in f (minimax for the
-// relative error, by Remez exchange: 2^-18.5) and i added to the exponent. Below -126 the result is about
-// 2^-126 instead of less.
-__device__ __forceinline__ f32x2 exp2_pair(f32x2 x) {
-  float a, b;
-  unpack2(x, a, b);
-  x = pack2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
-  const f32x2 magic = pack2(12582912.0f, 12582912.0f);  // 1.5 * 2^23: the sum's last bits are round(x)
-  const f32x2 shifted = add2(x, magic);
-  const f32x2 f = add2(x, fma2(shifted, pack2(-1.0f, -1.0f), magic));
-  f32x2 r = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f, pack2(0.05591785907745361f, 0.05591785907745361f));
-  r = fma2(r, f, pack2(0.240247443318367f, 0.240247443318367f));
-  r = fma2(r, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-  r = fma2(r, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-  float ra, rb, sa, sb;
-  unpack2(r, ra, rb);
-  unpack2(shifted, sa, sb);
-  return pack2(__int_as_float(__float_as_int(ra) + (__float_as_int(sa) << 23)),
-               __int_as_float(__float_as_int(rb) + (__float_as_int(sb) << 23)));
-}
-
 // Two copies of mine / larger in fp16 (exactly 1 for the block that has the larger scale).
 __device__ __forceinline__ uint32_t scale_ratio(float mine, float larger) {
   const __half2 ratio = __float2half2_rn(larger > 0.0f ? __fdividef(mine, larger) : 0.0f);
@@ -340,120 +327,6 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     atomicExch(p.status, kStatusWaitTimeout);
   };
 
-  // ---- 8-bit tiles to 16 bits: 128 threads, tiles `begin`, `begin` + `stride`, ... of keys 2 j and values 2 j + 1
-  auto convert = [&](int t, int begin, int stride, auto barrier) {
-      constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
-      constexpr int kPasses = kTileTokens / kRowsPerPass;
-      // A thread's rows are first + pass * kRowsPerPass, a batch at a time: all loads, all arithmetic, all
-      // stores. (The loads and stores are volatile: in the order of one row after the other every row
-      // waits for the one before, 230 clocks each.)
-      constexpr int kBatch = 4;
-      uint32_t* key_ratios = reinterpret_cast<uint32_t*>(smem + L::kRatios);  // [8 pages][2 blocks]
-      uint32_t* value_ratios = key_ratios + 16;                               // [128 rows][2 blocks]
-      const int page_shift = p.page_size == 16 ? 4 : 5;
-      const int chunk = t % kChunks;
-      const int block = chunk / 8;
-      const int first = t / kChunks;
-      bool ok = true;
-      for (int i = begin; ok && i < 2 * count; i += stride) {
-        const int raw_slot = i % (QUANT ? L::kRawSlots : 1);
-        const int slot = i % L::kSlots;
-        const int raw_use = i / (QUANT ? L::kRawSlots : 1);
-        const int use = i / L::kSlots;
-        const int j = i >> 1;
-        const bool keys = (i & 1) == 0;
-        // In this order: with every other tile the group does not see a raw slot's every phase, but tile
-        // i - kSlots being released says that the copies before this one have landed, so that the parity
-        // can only mean this one.
-        static_assert(!QUANT || L::kRawSlots >= L::kSlots, "a raw slot's previous tile is released with the operand slot's");
-        ok = (use == 0 || wait_for(empty + 8 * slot, (use - 1) & 1)) && wait_for(raw_full + 8 * raw_slot, raw_use & 1);
-        if (!ok) {
-          break;
-        }
-        const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
-        const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
-        const int valid = min(kTileTokens, loaded - j * kTileTokens);
-        const uint32_t* ratios = keys ? key_ratios : value_ratios;
-        if (keys) {
-          if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
-            const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + t * 8);
-            const float larger = fmaxf(s.x, s.y);
-            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + t] = larger;
-            if constexpr (kBlocks == 2) {
-              key_ratios[2 * t] = scale_ratio(s.x, larger);
-              key_ratios[2 * t + 1] = scale_ratio(s.y, larger);
-            }
-          }
-        } else {
-          // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
-          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes) + t * kBlocks;
-          float larger = scales[0];
-          if constexpr (kBlocks == 2) {
-            larger = fmaxf(larger, scales[1]);
-            value_ratios[2 * t] = scale_ratio(scales[0], larger);
-            value_ratios[2 * t + 1] = scale_ratio(scales[1], larger);
-          }
-          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
-          factors[0] = t < valid ? larger : 0.0f;
-          // (a scale of 0 must not leave a tile without a finite heaviest weight)
-          const float log = t < valid ? __log2f(fmaxf(larger, 1e-30f)) : -INFINITY;
-          factors[kFactorRing * kTileTokens] = log;
-          float most = log;
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) {
-            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
-          }
-          if (lane == 0) {
-            reinterpret_cast<float*>(smem + L::kTileLogs)[(j % kFactorRing) * 4 + (warp & 3)] = most;
-          }
-        }
-        if constexpr (kBlocks == 2) {
-          asm volatile("bar.sync %0, 128;" ::"n"(decltype(barrier)::value) : "memory");  // the ratios, by the rows' other threads
-        }
-#pragma unroll
-        for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
-          uint2 w[kBatch];
-          uint32_t ratio[kBatch];
-          uint4 out[kBatch];
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            const int row = first + (pass0 + b) * kRowsPerPass;
-            w[b] = lds64(from + row * D + chunk * 8);
-            ratio[b] = kBlocks == 2 ? ratios[(keys ? row >> page_shift : row) * 2 + block] : 0u;
-          }
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            const int row = first + (pass0 + b) * kRowsPerPass;
-            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out[b].x, out[b].y);
-            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out[b].z, out[b].w);
-            if constexpr (kBlocks == 2) {
-              out[b].x = mul_half2(out[b].x, ratio[b]);
-              out[b].y = mul_half2(out[b].y, ratio[b]);
-              out[b].z = mul_half2(out[b].z, ratio[b]);
-              out[b].w = mul_half2(out[b].w, ratio[b]);
-            }
-            // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
-            if (row >= valid) {
-              out[b] = make_uint4(0u, 0u, 0u, 0u);
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            sts128(to + operand_chunk(first + (pass0 + b) * kRowsPerPass, chunk), out[b]);
-          }
-        }
-        proxy_fence_async();
-        __syncwarp();
-        if (lane == 0) {
-          umma::mbar_arrive(full + 8 * slot);
-          umma::mbar_arrive(raw_empty + 8 * raw_slot);
-        }
-      }
-      if (!ok) {
-        give_up();
-      }
-  };
-
   if (warp < 8) {
     tile::registers_up<L::kSoftmaxRegisters>();
     const int x = warp >> 2;
@@ -558,11 +431,6 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         umma::mbar_arrive(q_ready);
       }
       asm volatile("bar.sync 1, 256;" ::: "memory");  // row_power is read by other warps than its writers
-    }
-    if constexpr (QUANT) {
-      if (x == 1 && tiles[1] == 0 && count > 0) {  // no rows of its own: the values are converted here
-        convert(tid - 128, 1, 2, std::integral_constant<int, 3>{});
-      }
     }
     // ---- softmax --------------------------------------------------------------------------------
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -686,7 +554,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       const f32x2 minus_ref = pack2(-ref, -ref);
       f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
       auto probabilities = [&](auto all_seen) {  // in two instances: the compiler leaves the branch in otherwise
-        constexpr bool kAllSeen = decltype(all_seen)::value;
+        [[maybe_unused]] constexpr bool kAllSeen = decltype(all_seen)::value;
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         take(c, all_seen);
@@ -702,21 +570,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
             e = add2(pair_of(s + i), minus_ref);
           }
           float a, b;
-          if constexpr (!QUANT && kAllSeen) {
-            if (i % 8 == 6) {
-              unpack2(exp2_pair(e), a, b);
-            } else {
-              unpack2(e, a, b);
-              a = fk_page_decode::exp2_quick(a);
-              b = fk_page_decode::exp2_quick(b);
-            }
-          } else {
-            unpack2(e, a, b);
-            a = fk_page_decode::exp2_quick(a);
-            b = fk_page_decode::exp2_quick(b);
-          }
-          s[i] = __float_as_uint(a);
-          s[i + 1] = __float_as_uint(b);
+          unpack2(e, a, b);
+          s[i] = __float_as_uint(fk_page_decode::exp2_quick(a));
+          s[i + 1] = __float_as_uint(fk_page_decode::exp2_quick(b));
         }
 #pragma unroll
         for (int i = 0; i < 32; i += 4) {
@@ -1028,8 +884,114 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         give_up();
       }
     } else if (QUANT && warp >= 12 && count > 0) {
-      if constexpr (QUANT) {
-        convert(tid - 384, 0, tiles[1] > 0 ? 1 : 2, std::integral_constant<int, 2>{});
+      // ---- 8-bit tiles to 16 bits ---------------------------------------------------------------
+      constexpr int kRowsPerPass = 128 / kChunks;  // 128 threads, 8 elements each
+      constexpr int kPasses = kTileTokens / kRowsPerPass;
+      // A thread's rows are first + pass * kRowsPerPass, a batch at a time: all loads, all arithmetic, all
+      // stores. (The loads and stores are volatile: in the order of one row after the other every row
+      // waits for the one before, 230 clocks each.)
+      constexpr int kBatch = 4;
+      uint32_t* key_ratios = reinterpret_cast<uint32_t*>(smem + L::kRatios);  // [8 pages][2 blocks]
+      uint32_t* value_ratios = key_ratios + 16;                               // [128 rows][2 blocks]
+      constexpr int kRawSlots = QUANT ? L::kRawSlots : 1;
+      const int t = tid - 384;
+      const int page_shift = p.page_size == 16 ? 4 : 5;
+      const int chunk = t % kChunks;
+      const int block = chunk / 8;
+      const int first = t / kChunks;
+      bool ok = true;
+      for (int i = 0; ok && i < 2 * count; ++i) {
+        const int raw_slot = i % kRawSlots;
+        const int slot = i % L::kSlots;
+        const int raw_use = i / kRawSlots;
+        const int use = i / L::kSlots;
+        const int j = i >> 1;
+        const bool keys = (i & 1) == 0;
+        ok = (use == 0 || wait_for(empty + 8 * slot, (use - 1) & 1)) && wait_for(raw_full + 8 * raw_slot, raw_use & 1);
+        if (!ok) {
+          break;
+        }
+        const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
+        const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
+        const int valid = min(kTileTokens, loaded - j * kTileTokens);
+        const uint32_t* ratios = keys ? key_ratios : value_ratios;
+        if (keys) {
+          if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
+            const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + t * 8);
+            const float larger = fmaxf(s.x, s.y);
+            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + t] = larger;
+            if constexpr (kBlocks == 2) {
+              key_ratios[2 * t] = scale_ratio(s.x, larger);
+              key_ratios[2 * t + 1] = scale_ratio(s.y, larger);
+            }
+          }
+        } else {
+          // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
+          const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes) + t * kBlocks;
+          float larger = scales[0];
+          if constexpr (kBlocks == 2) {
+            larger = fmaxf(larger, scales[1]);
+            value_ratios[2 * t] = scale_ratio(scales[0], larger);
+            value_ratios[2 * t + 1] = scale_ratio(scales[1], larger);
+          }
+          float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
+          factors[0] = t < valid ? larger : 0.0f;
+          // (a scale of 0 must not leave a tile without a finite heaviest weight)
+          const float log = t < valid ? __log2f(fmaxf(larger, 1e-30f)) : -INFINITY;
+          factors[kFactorRing * kTileTokens] = log;
+          float most = log;
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) {
+            most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+          }
+          if (lane == 0) {
+            reinterpret_cast<float*>(smem + L::kTileLogs)[(j % kFactorRing) * 4 + (warp & 3)] = most;
+          }
+        }
+        if constexpr (kBlocks == 2) {
+          asm volatile("bar.sync 2, 128;" ::: "memory");  // the ratios, by the rows' other threads
+        }
+#pragma unroll
+        for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
+          uint2 w[kBatch];
+          uint32_t ratio[kBatch];
+          uint4 out[kBatch];
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = first + (pass0 + b) * kRowsPerPass;
+            w[b] = lds64(from + row * D + chunk * 8);
+            ratio[b] = kBlocks == 2 ? ratios[(keys ? row >> page_shift : row) * 2 + block] : 0u;
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int row = first + (pass0 + b) * kRowsPerPass;
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out[b].x, out[b].y);
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out[b].z, out[b].w);
+            if constexpr (kBlocks == 2) {
+              out[b].x = mul_half2(out[b].x, ratio[b]);
+              out[b].y = mul_half2(out[b].y, ratio[b]);
+              out[b].z = mul_half2(out[b].z, ratio[b]);
+              out[b].w = mul_half2(out[b].w, ratio[b]);
+            }
+            // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
+            if (row >= valid) {
+              out[b] = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            sts128(to + operand_chunk(first + (pass0 + b) * kRowsPerPass, chunk), out[b]);
+          }
+        }
+        proxy_fence_async();
+        __syncwarp();
+        if (lane == 0) {
+          umma::mbar_arrive(full + 8 * slot);
+          umma::mbar_arrive(raw_empty + 8 * raw_slot);
+        }
+      }
+      if (!ok) {
+        give_up();
       }
     }
   }

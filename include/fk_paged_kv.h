@@ -96,15 +96,21 @@ typedef struct fk_paged_kv_append_args {
  * vectors and kv head. Otherwise it leaves, per vector and query head, the weighted values, the
  * maximum of the logits in units of ln 2 and the denominator at
  *     partials[(first partial of the vector + partial result of the item) * num_q_heads + q_head]
- * (rows of head_dim + 4 floats: values, maximum, denominator, two unused). With `combine` != 0 a second
+ * (rows of head_dim + 4 floats: values, maximum, denominator, two unused; any number serves as the maximum
+ * that values and denominator are relative to). With `combine` != 0 a second
  * kernel adds the partial results of every vector that has some, in order, into `output`; without it
  * the caller hands them to fk_page_decode_forward_merged.
  *
- * Rounding. Logits, maxima, denominators and weighted values are fp32. The turned query is rounded to
- * 16 bits once (bf16 pages: bf16; 8-bit pages: fp16 behind an exact power of two), probabilities to
- * bf16 once, against keys and values as they are stored (8-bit values times their token's scale relative
- * to the token's larger one: bf16). A non-finite key or value of a token that counts may reach every
- * vector of an item; what lies behind a request's last token is never used. */
+ * The positions of a causal item's vectors ascend. An item that does not fit the arrays is left out.
+ *
+ * Rounding. Logits, maxima, denominators and weighted values are fp32. bf16 pages: the turned query and the
+ * probabilities are rounded to bf16 once. 8-bit pages: the turned query is rounded to fp16 behind an
+ * exact power of two; keys and values are fp16 numbers, exact in the 64-dim block that has the page's
+ * (token's) larger scale, the other block's times the ratio of the two scales; a probability times its
+ * token's larger value scale is rounded to fp16 relative to the row's heaviest, so that one below 2^-14
+ * of it is off by up to 2^-25 of it. A non-finite key or value of a token that counts may reach every
+ * vector of an item; what lies behind a request's last token is never used. Results do not depend on
+ * timing. */
 #define FK_PAGED_KV_ITEM_ROWS 256
 typedef struct fk_paged_kv_attention_args {
   const void* query; /* bf16 rows [rows][num_q_heads][head_dim], strides below, 16-byte aligned rows */

@@ -275,3 +275,70 @@ def test_attention_plan_refusals() -> None:
                             ({"page_table": torch.zeros((0, 2), dtype=torch.int32), "seq_lens": torch.zeros(0, dtype=torch.int32)}, "empty")):
         with pytest.raises(ValueError, match=message):
             plan(**{**arguments, **change})
+
+
+# ---- the entry points refuse before they touch the device ----------------------------------------------------
+
+
+def test_native_attention_checks_its_arguments_before_the_device() -> None:
+    from fast_kernels.native import native_module
+
+    call = native_module().paged_attention_forward
+    good = dict(query_ptr=256, query_row_stride=256, query_head_stride=64, key_ptr=256, value_ptr=256, key_scales_ptr=256,
+                value_scales_ptr=256, page_ids_ptr=256, vectors_ptr=256, items_ptr=256, output_ptr=256, partials_ptr=256, num_rows=1,
+                num_page_ids=1, num_vectors=1, num_items=1, num_partials=1, num_pages=1, num_q_heads=4, num_kv_heads=2, head_dim=64,
+                page_size=16, kv_format=2, softmax_scale=0.1, rope_theta=10000.0, stream_ptr=0)
+    call(**{**good, "num_items": 0, "query_ptr": 0})  # nothing to do
+    call(**{**good, "num_vectors": 0, "query_ptr": 0})
+    for change, message in (({"head_dim": 96}, "head_dim"), ({"page_size": 8}, "page_size"), ({"kv_format": 3}, "kv_format"),
+                            ({"num_q_heads": 3}, "divisible"), ({"num_q_heads": 1024}, "256 query heads"), ({"num_rows": -1}, "non-negative"),
+                            ({"softmax_scale": float("nan")}, "softmax_scale"), ({"rope_theta": -1.0}, "rope_theta"),
+                            ({"query_ptr": 0}, "NULL"), ({"items_ptr": 0}, "NULL"), ({"partials_ptr": 0}, "partials"),
+                            ({"key_scales_ptr": 0}, "scales"), ({"output_ptr": 264}, "aligned"), ({"key_scales_ptr": 260}, "aligned"),
+                            ({"query_row_stride": 12}, "multiples of 8"), ({"num_pages": 0}, "num_pages"),
+                            ({"num_pages": 2**30}, "31 bits"), ({"num_vectors": 2**30}, "31 bits")):
+        with pytest.raises(ValueError, match=message):
+            call(**{**good, **change})
+
+
+def test_native_shared_decode_wants_items_with_partial_results() -> None:
+    from fast_kernels.native import native_module
+
+    call = native_module().shared_prefix_decode_forward
+    pointers = {f"{name}_ptr": 256 for name in (
+        "query", "key", "value", "key_scales", "value_scales", "page_ids", "vectors", "items", "of_request", "run_base_pages",
+        "run_page_counts", "run_logical_starts", "run_last_page_lens", "request_run_offsets", "seq_lens", "output", "partials")}
+    good = dict(**pointers, batch=1, num_page_ids=1, num_items=1, num_partials=1, num_runs=0, max_tail_pages=0, num_pages=1,
+                num_q_heads=4, num_kv_heads=2, head_dim=64, page_size=16, kv_format=0, softmax_scale=0.1, rope_theta=10000.0, stream_ptr=0)
+    for change, message in (({"num_partials": 0}, "come together"), ({"num_items": 0}, "come together"), ({"num_items": -1}, "come together"),
+                            ({"head_dim": 32}, "head_dim"), ({"num_kv_heads": 0}, "divisible")):
+        with pytest.raises(ValueError, match=message):
+            call(**{**good, **change})
+
+
+def test_merged_decode_checks_the_prior_rows() -> None:
+    from fast_kernels import page_decode_capi as pdc
+
+    lib, args = pdc.load_library(), pdc.PageDecodeArgs()
+    for rows, of_request, message in ((0, 256, "NULL"), (256, 0, "NULL"), (264, 256, "aligned"), (256, 260, "aligned"), (256, 256, "empty inputs")):
+        prior = pdc.PageDecodePrior(rows, of_request)
+        assert lib.fk_page_decode_forward_merged(ctypes.byref(args), ctypes.byref(prior)) == pdc.ERR_INVALID_ARGUMENT
+        assert message in lib.fk_page_decode_last_error().decode()
+    assert lib.fk_page_decode_forward_merged(ctypes.byref(args), None) == pdc.ERR_INVALID_ARGUMENT
+
+
+def test_a_build_without_cuda_has_the_names(tmp_path: Path) -> None:
+    import importlib.util
+    import subprocess
+    import sys
+
+    spec = importlib.util.spec_from_file_location("fk_build", REPO / "fast-kernels_b200" / "build.py")
+    build = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(build)
+    build.build_python_module_without_cuda(tmp_path)
+    child = ("import sys; sys.path.insert(0, sys.argv[1]); import _native\n"
+             "for name in ('paged_kv_append_forward', 'paged_attention_forward', 'shared_prefix_decode_forward'): assert hasattr(_native, name)\n"
+             "try: _native.paged_kv_device_status()\n"
+             "except RuntimeError as error: print(error)")
+    done = subprocess.run([sys.executable, "-c", child, str(tmp_path)], capture_output=True, text=True, check=True)
+    assert done.stdout.strip() == "fast-kernels was built without CUDA support"
