@@ -48,8 +48,13 @@ def host_ints(tensor: Any, name: str, ndim: int) -> np.ndarray:
 
 
 def table_and_lengths(page_table: Any, **lengths: Any) -> list[np.ndarray]:
-    """The page table and 1D length tensors as int64 arrays, one non-negative length per request."""
-    table = host_ints(page_table, "page_table", 2)
+    """The page table (int32 as it mostly comes, or int64) and 1D length tensors as int64 arrays, one non-negative length
+    per request."""
+    torch = _torch()
+    if isinstance(page_table, torch.Tensor) and page_table.dtype == torch.int32 and page_table.ndim == 2:
+        table = page_table.detach().cpu().contiguous().numpy()
+    else:
+        table = host_ints(page_table, "page_table", 2)
     out = [table]
     for name, tensor in lengths.items():
         values = host_ints(tensor, name, 1)
@@ -70,7 +75,7 @@ def require_pages(table: np.ndarray, request: np.ndarray, slot: np.ndarray) -> n
     pages = table[request, slot]
     if pages.size and int(pages.min()) < 0:
         raise ValueError("page_table has no page for some of the tokens")
-    if pages.size and int(pages.max()) >= 1 << 31:
+    if pages.dtype != np.int32 and pages.size and int(pages.max()) >= 1 << 31:
         raise ValueError("page_table entries must fit 32 bits")
     return pages
 

@@ -17,21 +17,18 @@ def pieces_for(tiles: np.ndarray, kv_heads: int, fewest: int = 1) -> np.ndarray:
     if tiles.size == 0:
         return np.zeros(0, dtype=np.int64)
     longest = int(tiles.max())
-    best, chosen = None, np.ones_like(tiles)
-    for cut in range(1, 65):
-        most = -(-longest // cut)
-        if cut > 1 and most < fewest:
-            break
-        pieces = -(-tiles // most)
-        size = -(-tiles // pieces)
-        items = int(pieces.sum()) * kv_heads
-        mean = float((pieces * size).sum()) / float(pieces.sum()) + _ITEM_OVERHEAD
-        if int(pieces.max()) > 1:
-            mean += 1  # partial results are written and added up
-        cost = max(float(size.max()) + _ITEM_OVERHEAD, -(-items // _SMS) * mean)
-        if best is None or cost < 0.97 * best:
-            best, chosen = cost, pieces
-    return chosen
+    most = -(-longest // np.arange(1, 65))  # tiles of a piece at most, for 1, 2, ... pieces of the longest
+    most = most[: max(1, int((most >= fewest).sum()))][:, None]
+    pieces = -(-tiles // most)
+    size = -(-tiles // pieces)
+    total = pieces.sum(axis=1)
+    mean = (pieces * size).sum(axis=1) / total + _ITEM_OVERHEAD + (pieces.max(axis=1) > 1)  # (partial results are added up)
+    costs = np.maximum(size.max(axis=1) + _ITEM_OVERHEAD, -(-(total * kv_heads) // _SMS) * mean).tolist()
+    chosen = 0
+    for index, cost in enumerate(costs):
+        if cost < 0.97 * costs[chosen]:
+            chosen = index
+    return pieces[chosen]
 
 
 def cut(first: np.ndarray, end: np.ndarray, pieces: np.ndarray) -> tuple[np.ndarray, np.ndarray, np.ndarray, np.ndarray]:

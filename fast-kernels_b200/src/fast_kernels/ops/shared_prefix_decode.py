@@ -86,9 +86,10 @@ def _shared_runs(table: np.ndarray, full_pages: np.ndarray, min_pages: int) -> t
     have in common; one shorter than `min_pages` is left to what comes further down."""
     batch = len(full_pages)
     width = int(full_pages.max()) if batch else 0
-    rows = np.where(np.arange(width) < full_pages[:, None], table[:, :width], -1 - np.arange(batch)[:, None])
-    keys = rows.astype(np.int64).astype(">i8") if width else np.zeros((batch, 1), dtype=">i8")
-    order = np.array(sorted(range(batch), key=lambda b: keys[b].tobytes()), dtype=np.int64)
+    fill = (-1 - np.arange(batch)).astype(table.dtype)[:, None]
+    rows = np.where(np.arange(width) < full_pages[:, None], table[:, :width], fill)
+    # (by their bytes: any order will do in which equal beginnings are neighbours)
+    order = np.array(sorted(range(batch), key=lambda b: rows[b].tobytes()), dtype=np.int64)
     rows = rows[order]
     same = rows[1:] == rows[:-1]
     common = np.where(same.all(axis=1), width, np.argmin(same, axis=1)) if width and batch > 1 else np.zeros(max(0, batch - 1), dtype=np.int64)
@@ -147,7 +148,7 @@ def _build(table: np.ndarray, lens: np.ndarray, num_q_heads: int, num_kv_heads: 
     used = table[slots < pages[:, None]]
     if used.size and int(used.min()) < 0:
         raise ValueError("page_table has no page for some of the tokens")
-    if used.size and int(used.max()) >= 1 << 31:
+    if used.dtype != np.int32 and used.size and int(used.max()) >= 1 << 31:
         raise ValueError("page_table entries must fit 32 bits")
     order, runs = _shared_runs(table, lens // page_size, -(-MIN_RUN_TOKENS // page_size))
     saved = sum((high - low - 1) * (end - first) for first, end, low, high in runs)
@@ -193,7 +194,7 @@ def _build(table: np.ndarray, lens: np.ndarray, num_q_heads: int, num_kv_heads: 
     for _, end, low, high in runs:
         covered[order[low:high]] = end
     rest = lens - covered * page_size
-    shifted = np.full((batch, max(1, int((-(-rest // page_size)).max()))), -1, dtype=np.int64)
+    shifted = np.full((batch, max(1, int((-(-rest // page_size)).max()))), -1, dtype=np.int32)
     column = np.arange(shifted.shape[1])
     take = column < (-(-rest // page_size))[:, None]
     shifted[take] = np.take_along_axis(table, np.minimum(column + covered[:, None], max(0, table.shape[1] - 1)), axis=1)[take] if table.shape[1] else 0
