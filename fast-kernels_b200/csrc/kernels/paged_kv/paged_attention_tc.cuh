@@ -343,42 +343,44 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       const int heads_each = (p.group + slices - 1) / slices;
       constexpr int kBatch = 4;  // heads whose loads are in flight together
       auto vector_of = [&](int task) -> int { return task < tasks ? (task / kChunks) % item.vectors : 0; };
-      int4 v = p.vectors[item.first_vector + vector_of(tid)];
+      auto descriptor = [&](int task) -> int4 { return __ldg(p.vectors + item.first_vector + vector_of(task)); };
+      // Heads h0 .. h0 + 3 of a task, as they are.
+      auto fetch = [&](int task, const int4& v, int h0, uint4 (&w)[kBatch]) {
+        const bool readable = task < tasks && v.x >= 0 && v.x < p.num_rows;
+        const int head0 = (task < tasks ? task / columns : 0) * heads_each;
+        const uint16_t* src = p.query + static_cast<long long>(readable ? v.x : 0) * p.query_row_stride +
+                              static_cast<long long>(item.kv_head * p.group + head0) * p.query_head_stride + (task % kChunks) * 8;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          w[b] = make_uint4(0u, 0u, 0u, 0u);
+          if (readable && h0 + b < heads_each && head0 + h0 + b < p.group) {
+            w[b] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(h0 + b) * p.query_head_stride));
+          }
+        }
+      };
+      int4 v = descriptor(tid), next_v = descriptor(tid + 256);
+      uint4 w[kBatch], next_w[kBatch];
+      fetch(tid, v, 0, w);
       for (int task = tid; task < round; task += 256) {
-        const bool active = task < tasks;
+        const int4 after_v = descriptor(task + 512);
+        fetch(task + 256, next_v, 0, next_w);
         const int chunk = task % kChunks;
         const int vector = vector_of(task);
-        const int slice = active ? task / columns : 0;
-        const bool readable = active && v.x >= 0 && v.x < p.num_rows;
-        const int position = v.y;
-        const uint16_t* src = p.query + static_cast<long long>(readable ? v.x : 0) * p.query_row_stride +
-                              static_cast<long long>(item.kv_head * p.group) * p.query_head_stride + chunk * 8;
-        v = p.vectors[item.first_vector + vector_of(task + 256)];
+        const int head0 = (task < tasks ? task / columns : 0) * heads_each;
         float2 cs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 turn = rope_cos_sin_quick(turns[chunk * 4 + i], v.y);
+          cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
+        }
         for (int h0 = 0; h0 < heads_each; h0 += kBatch) {
-          uint4 w[kBatch];
+          if (h0 > 0) {
+            fetch(task, v, h0, w);
+          }
+          uint4 out[kBatch];
+          int bits[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int head = slice * heads_each + h0 + b;
-            w[b] = make_uint4(0u, 0u, 0u, 0u);
-            if (readable && h0 + b < heads_each && head < p.group) {
-              w[b] = __ldg(reinterpret_cast<const uint4*>(src + static_cast<long long>(head) * p.query_head_stride));
-            }
-          }
-          if (h0 == 0) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 turn = rope_cos_sin_quick(turns[chunk * 4 + i], position);
-              cs[i] = make_float2(turn.x * p.scale_log2e, turn.y * p.scale_log2e);
-            }
-          }
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            if (h0 + b >= heads_each) {
-              break;
-            }
-            const int head = slice * heads_each + h0 + b;
-            const bool store = active && head < p.group;
             const uint32_t words[4] = {w[b].x, w[b].y, w[b].z, w[b].w};
             float q[8];
 #pragma unroll
@@ -387,8 +389,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
               q[2 * i] = even * cs[i].x - odd * cs[i].y;
               q[2 * i + 1] = even * cs[i].y + odd * cs[i].x;
             }
-            const int r = vector * p.group + head;
-            uint4 out;
+            bits[b] = 0;
             if constexpr (QUANT) {
               // fp16 has the precision but not the range: the row is divided by the power of two of its
               // largest element, which goes back on in fp32
@@ -401,20 +402,31 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
               for (int o = 1; o < kChunks; o <<= 1) {
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, o));
               }
-              const int bits = fk_page_decode::exponent_bits(largest);
-              const float shrink = fk_page_decode::inverse_power(bits);
-              out = make_uint4(pack_half(q[0] * shrink, q[1] * shrink), pack_half(q[2] * shrink, q[3] * shrink),
-                               pack_half(q[4] * shrink, q[5] * shrink), pack_half(q[6] * shrink, q[7] * shrink));
-              if (store && chunk == 0) {
-                row_power[r] = __int_as_float(bits);
-              }
+              bits[b] = fk_page_decode::exponent_bits(largest);
+              const float shrink = fk_page_decode::inverse_power(bits[b]);
+              out[b] = make_uint4(pack_half(q[0] * shrink, q[1] * shrink), pack_half(q[2] * shrink, q[3] * shrink),
+                                  pack_half(q[4] * shrink, q[5] * shrink), pack_half(q[6] * shrink, q[7] * shrink));
             } else {
-              out = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
-            }
-            if (store) {
-              sts128(base + L::kQueries + (r >> 7) * L::kOperandBytes + operand_chunk(r & 127, chunk), out);
+              out[b] = make_uint4(pack_bf16(q[0], q[1]), pack_bf16(q[2], q[3]), pack_bf16(q[4], q[5]), pack_bf16(q[6], q[7]));
             }
           }
+#pragma unroll
+          for (int b = 0; b < kBatch; ++b) {
+            const int head = head0 + h0 + b;
+            if (task < tasks && h0 + b < heads_each && head < p.group) {
+              const int r = vector * p.group + head;
+              if (QUANT && chunk == 0) {
+                row_power[r] = __int_as_float(bits[b]);
+              }
+              sts128(base + L::kQueries + (r >> 7) * L::kOperandBytes + operand_chunk(r & 127, chunk), out[b]);
+            }
+          }
+        }
+        v = next_v;
+        next_v = after_v;
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          w[b] = next_w[b];
         }
       }
       for (int idx = tid; idx < (256 - rows) * kChunks; idx += 256) {  // rows without a vector
