@@ -284,8 +284,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   if (warp == 8) {
     umma::tmem_alloc(bars, 512);
     umma::tmem_relinquish();
-  } else if (warp == 10) {
-    share_rope_table(p.rope, turns, D / 2, lane);
+  }
+  if (tid < D / 2) {
+    turns[tid] = p.rope.turns[tid];  // (a parameter indexed by the lane is read lane by lane: once is enough)
   }
   umma::fence_before_sync();
   __syncthreads();
@@ -342,12 +343,16 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       const int round = (tasks + 31) / 32 * 32;
       const int heads_each = (p.group + slices - 1) / slices;
       constexpr int kBatch = 4;  // heads whose loads are in flight together
-      auto vector_of = [&](int task) -> int { return task < tasks ? (task / kChunks) % item.vectors : 0; };
+      // (with one slice no division by a number that only the item knows; with more, a thread has one task)
+      auto vector_of = [&](int task) -> int {
+        return task >= tasks ? 0 : slices == 1 ? task / kChunks : (task / kChunks) % item.vectors;
+      };
+      auto slice_of = [&](int task) -> int { return task >= tasks || slices == 1 ? 0 : task / columns; };
       auto descriptor = [&](int task) -> int4 { return __ldg(p.vectors + item.first_vector + vector_of(task)); };
       // Heads h0 .. h0 + 3 of a task, as they are.
       auto fetch = [&](int task, const int4& v, int h0, uint4 (&w)[kBatch]) {
         const bool readable = task < tasks && v.x >= 0 && v.x < p.num_rows;
-        const int head0 = (task < tasks ? task / columns : 0) * heads_each;
+        const int head0 = slice_of(task) * heads_each;
         const uint16_t* src = p.query + static_cast<long long>(readable ? v.x : 0) * p.query_row_stride +
                               static_cast<long long>(item.kv_head * p.group + head0) * p.query_head_stride + (task % kChunks) * 8;
 #pragma unroll
@@ -366,7 +371,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         fetch(task + 256, next_v, 0, next_w);
         const int chunk = task % kChunks;
         const int vector = vector_of(task);
-        const int head0 = (task < tasks ? task / columns : 0) * heads_each;
+        const int head0 = slice_of(task) * heads_each;
         float2 cs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
