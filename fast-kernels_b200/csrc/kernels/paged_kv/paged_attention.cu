@@ -121,9 +121,14 @@ FK_PAGED_KV_API int fk_paged_kv_attention(const fk_paged_kv_attention_args* args
   }
   if (!aligned16(a.query) || !aligned16(a.key_pages) || !aligned16(a.value_pages) || !aligned16(a.vectors) ||
       !aligned16(a.items) || !aligned16(a.output) || !aligned16(a.partials) ||
-      (a.kv_format != kKvBf16 && (!aligned16(a.value_scales) || (reinterpret_cast<uintptr_t>(a.key_scales) & 7u) != 0))) {
+      (a.kv_format != kKvBf16 && !aligned16(a.value_scales))) {
     return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT,
-                "query, pages, value_scales, vectors, items, output and partials must be 16-byte aligned, key_scales 8-byte");
+                "query, pages, value_scales, vectors, items, output and partials must be 16-byte aligned");
+  }
+  // (a page's key scales are one load; a cache that starts inside another one's scales has no more alignment than that)
+  const uintptr_t scale_bytes = sizeof(float) * (a.head_dim / 64);
+  if (a.kv_format != kKvBf16 && (reinterpret_cast<uintptr_t>(a.key_scales) & (scale_bytes - 1)) != 0) {
+    return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT, "key_scales must be aligned to the head_dim / 64 scales of a page");
   }
   if (((a.query_row_stride | a.query_head_stride) & 7) != 0) {
     return fail(FK_PAGED_KV_ERR_INVALID_ARGUMENT, "strides of the query must be multiples of 8 elements");

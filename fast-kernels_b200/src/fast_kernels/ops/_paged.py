@@ -112,6 +112,8 @@ def on_device(kept: dict[int, Any], device: Any, stream: int, host: Callable[[],
     entry = kept.get(device.index)
     if entry is None:
         torch = _torch()
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("a plan's first call on a device uploads its tables: make one before the capture")
         tables = host()
         parts, starts, at = [], {}, 0
         for name, values in tables.items():

@@ -128,7 +128,8 @@ def paged_prompt_attention(
 ) -> Any:
     """`query` is bf16 [tokens, q_heads, head_dim], the requests' new tokens one request after the other (a view into
     a fused projection's rows will do), not yet turned by their positions. Either `query_lens` or a `plan` says how
-    many tokens each request has."""
+    many tokens each request has. A NaN or infinity in the keys or values of a request's tokens may reach the outputs of
+    all of that request's queries; pages behind its last token may hold anything."""
     torch = _torch()
     native = _paged.backend()
     if not isinstance(query, torch.Tensor):

@@ -262,6 +262,33 @@ def test_prompts_same_bits_every_time_on_streams_and_in_graphs() -> None:
     _status_ok()
 
 
+def test_prompts_over_a_slice_of_a_cache() -> None:
+    """All pages but the first, of one head: their scales start 4 bytes behind a boundary."""
+    table, pages = fragmented_table([3, 2], 1)
+    whole = random_cache(layout="int8_kv", pages=pages + 1, heads=1, page_size=16, dim=64, table=table, lens=[40, 32], theta=THETA, seed=4)
+    cache = dataclasses.replace(whole, **{name: getattr(whole, name)[1:] for name in ("key_pages", "value_pages", "key_scales", "value_scales")})
+    assert cache.key_scales.data_ptr() % 8 == 4
+    query = _query(12, 4, 64, 6)
+    rows = [(0, t) for t in range(30, 40)] + [(1, 30), (1, 31)]
+    _assert_rows(ops.paged_prompt_attention(query, cache, query_lens=torch.tensor([10, 2])), cache, query, rows, default_scale(64))
+    _status_ok()
+
+
+def test_first_calls_of_a_plan_are_refused_inside_a_capture() -> None:
+    table, pages = fragmented_table([3], 1)
+    cache = random_cache(layout="bf16_kv", pages=pages, heads=2, page_size=16, dim=64, table=table, lens=[40], theta=THETA, seed=4)
+    query = _query(3, 4, 64, 6)
+    plan = ops.plan_paged_prompt_attention(page_table=cache.page_table, seq_lens=cache.seq_lens, query_lens=torch.tensor([3]), num_q_heads=4,
+                                           num_kv_heads=2, head_dim=64, page_size=16, kv_layout="bf16_kv", use_cache=False)
+    output = torch.empty_like(query)
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        with pytest.raises(RuntimeError, match="before the capture"):
+            ops.paged_prompt_attention(query, cache, plan=plan, output=output)
+        output.zero_()
+    _assert_rows(ops.paged_prompt_attention(query, cache, plan=plan), cache, query, [(0, 37), (0, 38), (0, 39)], default_scale(64))
+    _status_ok()
+
+
 def test_prompts_empty_and_refused_calls() -> None:
     cache, query, _, got = _prompt("bf16_kv", [40], [3])
     assert ops.paged_prompt_attention(query[:0], cache, query_lens=torch.tensor([0])).shape == (0, 8, 128)

@@ -10,6 +10,7 @@ from pathlib import Path
 import numpy as np
 import pytest
 import torch
+from fast_kernels.ops import _paged
 from paged_kv_testlib import attention64, cache_values, fragmented_table, random_cache, rotate64
 
 REPO = Path(__file__).resolve().parent.parent
@@ -294,11 +295,32 @@ def test_native_attention_checks_its_arguments_before_the_device() -> None:
                             ({"num_q_heads": 3}, "divisible"), ({"num_q_heads": 1024}, "256 query heads"), ({"num_rows": -1}, "non-negative"),
                             ({"softmax_scale": float("nan")}, "softmax_scale"), ({"rope_theta": -1.0}, "rope_theta"),
                             ({"query_ptr": 0}, "NULL"), ({"items_ptr": 0}, "NULL"), ({"partials_ptr": 0}, "partials"),
-                            ({"key_scales_ptr": 0}, "scales"), ({"output_ptr": 264}, "aligned"), ({"key_scales_ptr": 260}, "aligned"),
-                            ({"query_row_stride": 12}, "multiples of 8"), ({"num_pages": 0}, "num_pages"),
+                            ({"key_scales_ptr": 0}, "scales"), ({"output_ptr": 264}, "aligned"), ({"key_scales_ptr": 258}, "aligned"),
+                            ({"key_scales_ptr": 260, "head_dim": 128}, "key_scales must be aligned"), ({"query_row_stride": 12}, "multiples of 8"), ({"num_pages": 0}, "num_pages"),
                             ({"num_pages": 2**30}, "31 bits"), ({"num_vectors": 2**30}, "31 bits")):
         with pytest.raises(ValueError, match=message):
             call(**{**good, **change})
+    # a cache that is a slice of another one starts at any of its pages' scales: the next check is what refuses this
+    for change in ({"key_scales_ptr": 260}, {"key_scales_ptr": 264, "head_dim": 128}):
+        with pytest.raises(ValueError, match="multiples of 8"):
+            call(**{**good, **change, "query_row_stride": 12})
+
+
+@pytest.mark.parametrize("first_call_captured", [True, False])
+def test_tables_of_a_plan_are_not_uploaded_into_a_capture(monkeypatch, first_call_captured: bool) -> None:
+    device = torch.device("cpu", 0)  # (an index is all that is asked of it)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    kept: dict = {}
+    if not first_call_captured:
+        before = _paged.on_device(kept, device, 0, lambda: {"a": np.arange(3), "b": np.arange(4)})
+        assert before["b"] - before["a"] == 512
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    if first_call_captured:
+        with pytest.raises(RuntimeError, match="before the capture"):
+            _paged.on_device(kept, device, 0, lambda: {"a": np.arange(3), "b": np.arange(4)})
+        assert not kept
+    else:
+        assert _paged.on_device(kept, device, 1, lambda: {}) == before
 
 
 def test_native_shared_decode_wants_items_with_partial_results() -> None:
