@@ -92,8 +92,8 @@ struct TcLayout {
   static constexpr int kKeyFactors = kRaw + kRawSlots * kRawSlotBytes;              // [ring][8 pages]
   static constexpr int kValueFactors = kKeyFactors + (kQuant ? kFactorRing * 32 : 0);  // [ring][128 tokens], then their log2
   static constexpr int kRawKeyScales = kValueFactors + (kQuant ? kFactorRing * 1024 : 0);  // [raw slot][8 pages][2]
-  static constexpr int kRatios = kRawKeyScales + kRawSlots * 64;                    // [8 pages + 128 tokens][2]
-  static constexpr int kTileLogs = kRatios + (kQuant ? 64 + 1024 : 0);              // [ring][4 warps]
+  static constexpr int kRatios = kRawKeyScales + kRawSlots * 64;                    // [keys, values][128 tokens][2]
+  static constexpr int kTileLogs = kRatios + (kQuant ? 2048 : 0);              // [ring][4 warps]
   static constexpr int kRowPower = kTileLogs + (kQuant ? kFactorRing * 16 : 0);     // [256]
   static constexpr int kTurns = kRowPower + (kQuant ? 1024 : 0);                    // [64]
   static constexpr int kBarriers = kTurns + 512;
@@ -908,8 +908,6 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       // stores. (The loads and stores are volatile: in the order of one row after the other every row
       // waits for the one before, 230 clocks each.)
       constexpr int kBatch = 4;
-      uint32_t* key_ratios = reinterpret_cast<uint32_t*>(smem + L::kRatios);  // [8 pages][2 blocks]
-      uint32_t* value_ratios = key_ratios + 16;                               // [128 rows][2 blocks]
       constexpr int kRawSlots = QUANT ? L::kRawSlots : 1;
       const int t = tid - 384;
       const int page_shift = p.page_size == 16 ? 4 : 5;
@@ -931,16 +929,18 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
         const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
         const int valid = min(kTileTokens, loaded - j * kTileTokens);
-        const uint32_t* ratios = keys ? key_ratios : value_ratios;
+        // [128 rows][2 blocks], keys' and values' apart: the next operand's are written while this one's are read. (A
+        // table of the keys' pages instead took four instructions more for every eight elements.)
+        uint2* ratios = reinterpret_cast<uint2*>(smem + L::kRatios) + (i & 1) * kTileTokens;
         if (keys) {
-          if (t < 8) {  // (a tile of larger pages has fewer: what lies behind is not used)
-            const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + t * 8);
-            const float larger = fmaxf(s.x, s.y);
-            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + t] = larger;
-            if constexpr (kBlocks == 2) {
-              key_ratios[2 * t] = scale_ratio(s.x, larger);
-              key_ratios[2 * t + 1] = scale_ratio(s.y, larger);
-            }
+          const int page = t >> page_shift;
+          const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + page * 8);
+          const float larger = fmaxf(s.x, s.y);
+          if ((t & (p.page_size - 1)) == 0) {
+            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + page] = larger;
+          }
+          if constexpr (kBlocks == 2) {
+            ratios[t] = make_uint2(scale_ratio(s.x, larger), scale_ratio(s.y, larger));
           }
         } else {
           // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
@@ -948,8 +948,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           float larger = scales[0];
           if constexpr (kBlocks == 2) {
             larger = fmaxf(larger, scales[1]);
-            value_ratios[2 * t] = scale_ratio(scales[0], larger);
-            value_ratios[2 * t + 1] = scale_ratio(scales[1], larger);
+            ratios[t] = make_uint2(scale_ratio(scales[0], larger), scale_ratio(scales[1], larger));
           }
           float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
           factors[0] = t < valid ? larger : 0.0f;
@@ -968,36 +967,38 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         if constexpr (kBlocks == 2) {
           asm volatile("bar.sync 2, 128;" ::: "memory");  // the ratios, by the rows' other threads
         }
+        const uint32_t* my_ratios = reinterpret_cast<const uint32_t*>(ratios + first) + block;
+        const uint32_t source = from + t * 8;
+        const uint32_t target = to + operand_chunk(first, chunk);  // (rows of a pass are a multiple of 8 further on)
 #pragma unroll
         for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
           uint2 w[kBatch];
           uint32_t ratio[kBatch];
-          uint4 out[kBatch];
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int row = first + (pass0 + b) * kRowsPerPass;
-            w[b] = lds64(from + row * D + chunk * 8);
-            ratio[b] = kBlocks == 2 ? ratios[(keys ? row >> page_shift : row) * 2 + block] : 0u;
+            w[b] = lds64(source + (pass0 + b) * kRowsPerPass * D);
+            ratio[b] = kBlocks == 2 ? my_ratios[(pass0 + b) * kRowsPerPass * 2] : 0u;
           }
 #pragma unroll
           for (int b = 0; b < kBatch; ++b) {
-            const int row = first + (pass0 + b) * kRowsPerPass;
-            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out[b].x, out[b].y);
-            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out[b].z, out[b].w);
+            uint4 out;
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].x, out.x, out.y);
+            fk_page_decode::bytes_to_half2<KV, false>(w[b].y, out.z, out.w);
             if constexpr (kBlocks == 2) {
-              out[b].x = mul_half2(out[b].x, ratio[b]);
-              out[b].y = mul_half2(out[b].y, ratio[b]);
-              out[b].z = mul_half2(out[b].z, ratio[b]);
-              out[b].w = mul_half2(out[b].w, ratio[b]);
+              out.x = mul_half2(out.x, ratio[b]);
+              out.y = mul_half2(out.y, ratio[b]);
+              out.z = mul_half2(out.z, ratio[b]);
+              out.w = mul_half2(out.w, ratio[b]);
             }
-            // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
-            if (row >= valid) {
-              out[b] = make_uint4(0u, 0u, 0u, 0u);
-            }
+            sts128(target + (pass0 + b) * kRowsPerPass * 128, out);
           }
-#pragma unroll
-          for (int b = 0; b < kBatch; ++b) {
-            sts128(to + operand_chunk(first + (pass0 + b) * kRowsPerPass, chunk), out[b]);
+        }
+        if (valid < kTileTokens) {
+          // a row behind the end has weight 0, but what its page holds there times 0 need not be 0
+          for (int row = first; row < kTileTokens; row += kRowsPerPass) {
+            if (row >= valid) {
+              sts128(to + operand_chunk(row, chunk), make_uint4(0u, 0u, 0u, 0u));
+            }
           }
         }
         proxy_fence_async();
