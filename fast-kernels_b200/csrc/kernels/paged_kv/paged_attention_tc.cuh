@@ -18,6 +18,11 @@
 // grown by more than kGrowth since the last time. The tensor core is done with O whenever a tile's logits
 // are: their commit follows the previous tile's second product.
 //
+// What the roles of a block execute side by side has to stay near the instruction cache: with the 8-bit pages'
+// conversion and the first pass for the maximum unrolled, 32768 tokens of fp8 took 449 us instead of 427, of
+// which a tenth of all issue slots' waits were for instructions. The exponentials are unrolled all the same
+// (rolled: no gain with 8-bit pages, 594 us instead of 577 with bf16).
+//
 // The exponentials are what the softmax warps are bound by (16 a clock and SM: 2048 clocks per token tile
 // and 256 rows, the two products take as long).
 //
@@ -473,41 +478,45 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       umma::fence_after_sync();
       const bool masked = (j + 1) * kTileTokens > unmasked[x];
       const int seen = limit - j * kTileTokens;
-      // QUANT: what 16 neighbouring logits are multiplied by, the page's key scale and the row's power of two
-      float factor[8];
+      // QUANT: what 16 neighbouring logits are multiplied by, the page's key scale and the row's power of two: from
+      // shared memory in the loops that are not unrolled, from registers for the exponentials
       const float4* value_factors = reinterpret_cast<const float4*>(smem + L::kValueFactors) + (j % kFactorRing) * 32;
       const float4* value_logs = value_factors + kFactorRing * 32;
+      const float* factors = reinterpret_cast<const float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
+      auto factor = [&](int g) -> float { return factors[p.page_size == 16 ? g : g >> 1] * power; };
+      float kept[8];
       if constexpr (QUANT) {
-        const float* factors = reinterpret_cast<const float*>(smem + L::kKeyFactors) + (j % kFactorRing) * 8;
 #pragma unroll
         for (int g = 0; g < 8; ++g) {
-          factor[g] = factors[p.page_size == 16 ? g : g >> 1] * power;
+          kept[g] = factor(g);
         }
       }
       uint32_t buffer[2][32];
       // Products of 32 tokens; with `masked` the logits, -inf where the row does not see the token.
-      auto take = [&](int c, auto all_seen) {
-        uint32_t(&s)[32] = buffer[c & 1];
+      auto take = [&](int c, uint32_t(&s)[32], uint32_t(&next)[32], auto all_seen) {
         tile::wait_ld32(s);
         if (c + 1 < 4) {
-          tile::ld32(s_tmem + 32 * (c + 1), buffer[(c + 1) & 1]);
+          tile::ld32(s_tmem + 32 * (c + 1), next);
         }
         if (!decltype(all_seen)::value && masked) {
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
-            const float logit = QUANT ? __uint_as_float(s[i]) * factor[2 * c + i / 16] : __uint_as_float(s[i]);
+            const float logit = QUANT ? __uint_as_float(s[i]) * factor(2 * c + i / 16) : __uint_as_float(s[i]);
             s[i] = c * 32 + i < seen ? __float_as_uint(logit) : 0xff800000u;
           }
         }
       };
-      auto factor_of = [&](int g) -> float { return masked ? 1.0f : factor[g]; };
+      auto factor_of = [&](int g) -> float { return masked ? 1.0f : factor(g); };
       // ---- the tile's largest logit ----
       float top = -INFINITY;
       tile::ld32(s_tmem, buffer[0]);
+#pragma unroll (QUANT ? 1 : 2)
+      for (int c0 = 0; c0 < 4; c0 += 2)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        take(c, std::false_type{});
-        uint32_t(&s)[32] = buffer[c & 1];
+      for (int u = 0; u < 2; ++u) {
+        const int c = c0 + u;
+        uint32_t(&s)[32] = buffer[u];
+        take(c, s, buffer[u ^ 1], std::false_type{});
         if constexpr (QUANT) {  // (scales are not negative)
           top = max3(top, largest_of<16>(s) * factor_of(2 * c), largest_of<16>(s + 16) * factor_of(2 * c + 1));
         } else {
@@ -527,10 +536,13 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           // the heaviest weight itself: the bound may be far above it
           top = -INFINITY;
           tile::ld32(s_tmem, buffer[0]);
+#pragma unroll 1
+          for (int c0 = 0; c0 < 4; c0 += 2)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            take(c, std::false_type{});
-            uint32_t(&s)[32] = buffer[c & 1];
+          for (int u = 0; u < 2; ++u) {
+            const int c = c0 + u;
+            uint32_t(&s)[32] = buffer[u];
+            take(c, s, buffer[u ^ 1], std::false_type{});
 #pragma unroll
             for (int i = 0; i < 32; i += 4) {
               const f32x2 f = pack2(factor_of(2 * c + i / 16), factor_of(2 * c + i / 16));
@@ -572,16 +584,19 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
       auto probabilities = [&](auto all_seen) {  // in two instances: the compiler leaves the branch in otherwise
         [[maybe_unused]] constexpr bool kAllSeen = decltype(all_seen)::value;
+#pragma unroll (QUANT || kAllSeen ? 2 : 1)
+      for (int c0 = 0; c0 < 4; c0 += 2)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        take(c, all_seen);
-        uint32_t(&s)[32] = buffer[c & 1];
+      for (int u = 0; u < 2; ++u) {
+        const int c = c0 + u;
+        uint32_t(&s)[32] = buffer[u];
+        take(c, s, buffer[u ^ 1], all_seen);
         uint32_t packed[16];
 #pragma unroll
         for (int i = 0; i < 32; i += 2) {
           f32x2 e;
           if constexpr (QUANT) {
-            const float f = kAllSeen ? factor[2 * c + i / 16] : 1.0f;
+            const float f = kAllSeen ? kept[2 * c + i / 16] : 1.0f;
             e = fma2(pair_of(s + i), pack2(f, f), minus_ref);
           } else {
             e = add2(pair_of(s + i), minus_ref);
@@ -611,7 +626,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           }
         }
         umma::st16(s_tmem + 16 * c, packed);
-        if (c & 1) {
+        if (u == 1) {
           umma::wait_st();
           umma::fence_before_sync();
           __syncwarp();
@@ -970,7 +985,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         const uint32_t* my_ratios = reinterpret_cast<const uint32_t*>(ratios + first) + block;
         const uint32_t source = from + t * 8;
         const uint32_t target = to + operand_chunk(first, chunk);  // (rows of a pass are a multiple of 8 further on)
-#pragma unroll
+#pragma unroll 1
         for (int pass0 = 0; pass0 < kPasses; pass0 += kBatch) {
           uint2 w[kBatch];
           uint32_t ratio[kBatch];
