@@ -39,14 +39,15 @@
 // the token's on the probability before it is rounded. (Values in bf16 with bf16 probabilities took five
 // times the conversion's instructions, and their two roundings made the error 1.5 times the output's own.)
 //
-// What it measures: 8192 tokens, 32 heads over 8 of 128, bf16, causal: 594 us, 925 TFLOP/s, 57 % of the
-// measured bf16 peak: a token tile takes 3450 clocks where the products need 2050. 512 tokens behind 32768
-// in fp8 pages, 32 heads over 4: 474 us, 584 TFLOP/s: bound by the conversion (3800 clocks a tile, in the
-// issue slots of the softmax warps) and the chain behind it.
+// What it measures: 8192 tokens, 32 heads over 8 of 128, bf16, causal: 574 us, 958 TFLOP/s, 59 % of the
+// measured bf16 peak: a token tile takes 3350 clocks where the products need 2050. 512 tokens behind 32768
+// in fp8 pages, 32 heads over 4: 427 us, 650 TFLOP/s, 5500 clocks a tile: bound by the conversion, in the
+// issue slots of the softmax warps, and the chain behind it.
 // Tried and slower: steps of 64 tokens with two buffers of logits per row tile (N = 64 costs the tensor
 // core as much as N = 128 when both operands come from shared memory: 748 us), four more converting warps
 // (fewer registers for the softmax: 602 us for 477), a quarter or half of the exponentials as polynomials
-// on the FMA pipe (613 and 640 us for 594).
+// on the FMA pipe (613 and 640 us for 594), the conversion in batches of two or eight rows a thread (444 and
+// 433 us for 427).
 #pragma once
 
 #include <cuda.h>
