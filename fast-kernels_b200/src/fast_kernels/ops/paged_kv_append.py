@@ -170,4 +170,5 @@ def paged_kv_append(
                 plan.num_tokens, cache.key_pages.shape[0], plan.num_kv_heads, plan.head_dim, plan.page_size,
                 _layout_id(plan.kv_layout), int(cache.keys_are_rotated),
                 float(cache.key_rope_theta) if cache.keys_are_rotated else 1.0, stream)
-    return dataclasses.replace(cache, seq_lens=plan.seq_lens_after_cpu)
+    # (a copy: the plan may be used again, and the caller may write to the cache's lengths)
+    return dataclasses.replace(cache, seq_lens=plan.seq_lens_after_cpu.clone())

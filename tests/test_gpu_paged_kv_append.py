@@ -171,6 +171,14 @@ def test_plan_none_and_empty_calls() -> None:
     assert torch.equal(after.key_pages, before.key_pages) and after.seq_lens.tolist() == [4, 0]
 
 
+def test_lengths_of_a_cache_are_its_own() -> None:
+    """A caller that ends a request by setting its length to 0 changes no other call with the same lengths."""
+    cache, keys, values = _case("bf16_kv", [4, 7], [2, 1])
+    new = torch.tensor([2, 1])
+    ops.paged_kv_append(keys, values, cache, append_lens=new).seq_lens.zero_()
+    assert ops.paged_kv_append(keys, values, cache, append_lens=new).seq_lens.tolist() == [6, 8]
+
+
 def test_two_streams_and_a_captured_step() -> None:
     """One plan on two streams into two caches, and a step replayed from a graph into pages that were changed since."""
     lens, new = [5, 33], [1, 1]
