@@ -123,7 +123,9 @@ def on_device(kept: dict[int, Any], device: Any, stream: int, host: Callable[[],
             at += 4 * (values.size + gap)
         block = torch.from_numpy(np.concatenate(parts)).to(device=device)
         base = block.data_ptr()
-        entry = kept[device.index] = (block, {name: base + start for name, start in starts.items()}, stream)
+        # (two host threads may both get here: the first entry stands, so that nobody is given addresses into a block
+        # that the other one's entry has just dropped)
+        entry = kept.setdefault(device.index, (block, {name: base + start for name, start in starts.items()}, stream))
     block, addresses, home = entry
     if stream != home:
         torch = _torch()
