@@ -29,7 +29,8 @@
 // Roles (warps): 0-3 and 4-7 softmax of the two row tiles (they also turn and store the queries, and
 // write the results), 8 and 11 issue the two tiles' MMAs, 9 the copies, 10 clears the value
 // rows behind the end (a probability of 0 times whatever a page holds there would not be 0). 8-bit pages:
-// 12-15 convert. Every wait is bounded.
+// 12-15 convert. Every wait is bounded, and a warp's lanes give up together (wait_all): what they do next
+// needs all of them. Barriers that have no limit (bar.sync) are reached on every path.
 //
 // Operands in shared memory are rows of 128 bytes (64 16-bit elements) under the 128-byte swizzle; a
 // tile of 128-dimensional rows is two such halves. bf16 pages are copied there by TMA, one box of
@@ -122,6 +123,11 @@ __device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity) {
       : "r"(bar), "r"(parity)
       : "memory");
   return done != 0 || mbar_wait_parked(bar, parity);
+}
+// The same by a whole warp: one verdict for all lanes. Each lane's limit runs out by its own clock, and lanes
+// that went different ways would meet shuffles, tensor memory loads and barriers with members missing.
+__device__ __forceinline__ bool wait_all(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, wait_for(bar, parity));
 }
 
 __device__ __forceinline__ void mma_f16_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
@@ -262,9 +268,11 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   const uint32_t raw_empty = raw_full + 8 * 8;
   volatile uint32_t* fail_flag = reinterpret_cast<volatile uint32_t*>(smem + L::kBarriers + 8);
   volatile uint32_t* tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + L::kBarriers);
+  volatile int* issued_slot = reinterpret_cast<volatile int*>(smem + L::kBarriers + 12);  // operand copies begun
 
   if (tid == 0) {
     *fail_flag = 0u;
+    *issued_slot = 0;
     mbar_init(q_ready, 8);
     for (int x = 0; x < 2; ++x) {
       mbar_init(s_ready + 8 * x, 1);
@@ -471,7 +479,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < tiles[x]; ++j) {
-      ok = wait_for(s_ready + 8 * x, j & 1);
+      ok = wait_all(s_ready + 8 * x, j & 1);
       if (!ok) {
         give_up();
         break;
@@ -526,7 +534,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       }
       if constexpr (QUANT) {
         const int index = 2 * j + 1;  // the value scales come with the tile's values
-        ok = wait_for(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
+        ok = wait_all(full + 8 * (index % L::kSlots), (index / L::kSlots) & 1);
         if (!ok) {
           give_up();
           break;
@@ -652,12 +660,12 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     // Every thread lays its row out in shared memory (once both row tiles are done with the operands there)
     // and a bulk copy takes it away: stores straight from a thread per row touch 32 lines an instruction,
     // 9000 clocks for 256 rows of partial results.
-    if (tiles[x] > 0 && ok && !wait_for(o_final + 8 * x, 0)) {
+    if (tiles[x] > 0 && ok && !wait_all(o_final + 8 * x, 0)) {
       give_up();
       ok = false;
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (ok && x * kTileRows < rows && fits && *fail_flag == 0u) {
+    if (ok && x * kTileRows < rows && fits && __all_sync(0xffffffffu, *fail_flag == 0u)) {
       umma::fence_after_sync();
       const bool direct = item.partial < 0;
       const bool write_row = r < rows && vec.x >= 0 && vec.x < p.num_rows &&
@@ -835,7 +843,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         const int here = min(pages_per_tile, pages - j * pages_per_tile);  // pages of this tile
         for (int which = 0; which < 2; ++which) {  // keys, then values
           if (uses > 0) {
-            ok = wait_for(bars_empty + 8 * slot, (uses - 1) & 1);
+            ok = wait_all(bars_empty + 8 * slot, (uses - 1) & 1);
             if (!ok) {
               break;
             }
@@ -888,21 +896,18 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         key_scale = next_scale;
         next_page = after_page;
       }
+      if (lane == 0) {
+        *issued_slot = issued;
+      }
       if (!ok) {
         give_up();
-        // let the copies in flight land before the shared memory is handed on
-        for (int i = max(0, issued - kSlotCount); i < issued; ++i) {
-          if (!wait_for(bars_full + 8 * (i % kSlotCount), (i / kSlotCount) & 1)) {
-            break;
-          }
-        }
       }
     } else if (!QUANT && warp == 10 && clear_needed) {
       // ---- value rows behind the end ------------------------------------------------------------
       // The issuer says when they have landed: it follows the ring's phases one by one, and a wait for
       // a later phase's parity would be over at once.
       const int slot = (2 * count - 1) % L::kSlots;  // the last tile's values, in the order of the copies
-      if (wait_for(v_landed, 0)) {
+      if (wait_all(v_landed, 0)) {
         const int valid = loaded - (count - 1) * kTileTokens;
         const uint32_t v_base = base + L::kRing + slot * L::kOperandBytes;
         for (int idx = lane; idx < (kTileTokens - valid) * kChunks; idx += 32) {
@@ -930,25 +935,23 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       const int chunk = t % kChunks;
       const int block = chunk / 8;
       const int first = t / kChunks;
+      // A warp that gives up goes on through the loop, as far as the barrier that it shares with the others.
       bool ok = true;
-      for (int i = 0; ok && i < 2 * count; ++i) {
+      for (int i = 0; i < 2 * count; ++i) {
         const int raw_slot = i % kRawSlots;
         const int slot = i % L::kSlots;
         const int raw_use = i / kRawSlots;
         const int use = i / L::kSlots;
         const int j = i >> 1;
         const bool keys = (i & 1) == 0;
-        ok = (use == 0 || wait_for(empty + 8 * slot, (use - 1) & 1)) && wait_for(raw_full + 8 * raw_slot, raw_use & 1);
-        if (!ok) {
-          break;
-        }
+        ok = ok && (use == 0 || wait_all(empty + 8 * slot, (use - 1) & 1)) && wait_all(raw_full + 8 * raw_slot, raw_use & 1);
         const uint32_t from = base + L::kRaw + raw_slot * L::kRawSlotBytes;
         const uint32_t to = base + L::kRing + slot * L::kOperandBytes;
         const int valid = min(kTileTokens, loaded - j * kTileTokens);
         // [128 rows][2 blocks], keys' and values' apart: the next operand's are written while this one's are read. (A
         // table of the keys' pages instead took four instructions more for every eight elements.)
         uint2* ratios = reinterpret_cast<uint2*>(smem + L::kRatios) + (i & 1) * kTileTokens;
-        if (keys) {
+        if (ok && keys) {
           const int page = t >> page_shift;
           const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + page * 8);
           const float larger = fmaxf(s.x, s.y);
@@ -958,7 +961,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           if constexpr (kBlocks == 2) {
             ratios[t] = make_uint2(scale_ratio(s.x, larger), scale_ratio(s.y, larger));
           }
-        } else {
+        } else if (ok) {
           // row t's larger scale, and what softmax adds to the logit to know the heaviest weight
           const float* scales = reinterpret_cast<const float*>(smem + L::kRaw + raw_slot * L::kRawSlotBytes + L::kRawBytes) + t * kBlocks;
           float larger = scales[0];
@@ -982,6 +985,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         }
         if constexpr (kBlocks == 2) {
           asm volatile("bar.sync 2, 128;" ::: "memory");  // the ratios, by the rows' other threads
+        }
+        if (!ok) {
+          continue;
         }
         const uint32_t* my_ratios = reinterpret_cast<const uint32_t*>(ratios + first) + block;
         const uint32_t source = from + t * 8;
@@ -1034,14 +1040,23 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   umma::fence_before_sync();
   __syncthreads();
   umma::fence_after_sync();
-  if (*fail_flag != 0u && (warp == 8 || warp == 11) && lane == 0) {
-    umma::commit(drain);  // MMAs still in flight, if any
-  }
-  __syncwarp();
-  if (warp == 8) {
-    if (*fail_flag != 0u) {
-      (void)wait_for(drain, 0);
+  if (*fail_flag != 0u) {
+    // whatever is in flight still is let land before the memory is handed on: products, copies
+    if ((warp == 8 || warp == 11) && lane == 0) {
+      umma::commit(drain);
     }
+    __syncwarp();
+    if (warp == 8) {
+      (void)wait_all(drain, 0);
+    } else if (warp == 9) {
+      constexpr int kSlotCount = QUANT ? L::kRawSlots : L::kSlots;
+      const int issued = *issued_slot;
+      for (int i = max(0, issued - kSlotCount); i < issued; ++i) {
+        (void)wait_all((QUANT ? raw_full : full) + 8 * (i % kSlotCount), (i / kSlotCount) & 1);
+      }
+    }
+  }
+  if (warp == 8) {
     umma::tmem_dealloc(tmem, 512);
   }
 }
