@@ -3,6 +3,7 @@ of a plan on its devices, and plans remembered by their contents."""
 
 from __future__ import annotations
 
+import threading
 from collections import OrderedDict
 from contextlib import nullcontext
 from typing import Any, Callable
@@ -21,6 +22,8 @@ _ROW_ALIGN = 16  # bytes
 _UPLOAD_ALIGN = 128  # int32 words: 512 bytes
 _backend: Any = None
 _HERE = nullcontext()
+_REMEMBERING = threading.Lock()
+_IN_GRAPHS: dict[int, Any] = {}  # plans by identity
 
 
 def require_geometry(*, num_kv_heads: int, head_dim: int, page_size: int, kv_layout: str, num_q_heads: int | None = None) -> str:
@@ -80,17 +83,31 @@ def require_pages(table: np.ndarray, request: np.ndarray, slot: np.ndarray) -> n
     return pages
 
 
-def remembered(plans: OrderedDict, made_from: tuple, build: Callable[[], Any], use_cache: bool, most: int = 256) -> Any:
-    """A plan by the contents that it was made from; the `most` last ones are kept."""
+def remembered(plans: OrderedDict, made_from: tuple, build: Callable[[], Any], use_cache: bool, most: int = 32) -> Any:
+    """A plan by the contents that it was made from; the `most` last used ones are kept. (The lengths of a decode step never
+    come back, so nearly all plans of a server are dead after their step, each with its page table and device tables.)"""
     if not use_cache:
         return build()
     key = tuple((v.shape, v.tobytes()) if isinstance(v, np.ndarray) else v for v in made_from)
-    plan = plans.get(key)
-    if plan is None:
-        plan = plans[key] = build()
+    with _REMEMBERING:
+        plan = plans.get(key)
+        if plan is not None:
+            plans.move_to_end(key)
+            return plan
+    plan = build()
+    with _REMEMBERING:
+        plan = plans.setdefault(key, plan)
+        plans.move_to_end(key)
         while len(plans) > most:
             plans.popitem(last=False)
     return plan
+
+
+def keep_for_graphs(plan: Any) -> None:
+    """For a call that found its plan by itself: where it is being captured, the graph's replays read the plan's tables, and
+    nobody but this module can keep them. (A plan that the caller gave is the caller's to keep.)"""
+    if _torch().cuda.is_current_stream_capturing():
+        _IN_GRAPHS[id(plan)] = plan
 
 
 def backend() -> Any:

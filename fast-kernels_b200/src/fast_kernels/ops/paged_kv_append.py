@@ -146,6 +146,7 @@ def paged_kv_append(
     `append_lens` or a `plan` says how many tokens each request gets. Returns the cache with the new
     `seq_lens`; its pages are the same tensors."""
     native = _paged.backend()
+    found = plan is None
     if plan is None:
         if append_lens is None:
             raise ValueError("paged_kv_append needs append_lens or a plan")
@@ -163,6 +164,8 @@ def paged_kv_append(
     if plan.num_tokens:
         with _paged.current(device):
             stream = _paged.current_stream(device)
+            if found:
+                _paged.keep_for_graphs(plan)
             native.paged_kv_append_forward(
                 keys.data_ptr(), values.data_ptr(), *_paged.row_strides(keys), *_paged.row_strides(values),
                 cache.key_pages.data_ptr(), cache.value_pages.data_ptr(), _paged.address(cache.key_scales),

@@ -136,6 +136,7 @@ def paged_prompt_attention(
         raise TypeError("query must be a torch.Tensor")
     if query.ndim != 3:
         raise ValueError("query must be 3D")
+    found = plan is None
     if plan is None:
         if query_lens is None:
             raise ValueError("paged_prompt_attention needs query_lens or a plan")
@@ -156,6 +157,8 @@ def paged_prompt_attention(
         scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(plan.head_dim)
         with _paged.current(device):
             stream = _paged.current_stream(device)
+            if found:
+                _paged.keep_for_graphs(plan)
             tables = plan.device_tables(device, stream)
             partials = None
             if plan.num_partials:

@@ -227,6 +227,7 @@ def shared_prefix_decode(
         raise TypeError("query must be a torch.Tensor")
     if query.ndim != 3:
         raise ValueError("query must be 3D")
+    found = plan is None
     if plan is None:
         plan = plan_shared_prefix_decode(
             page_table=cache.page_table, seq_lens=cache.seq_lens, num_q_heads=int(query.shape[1]),
@@ -242,6 +243,8 @@ def shared_prefix_decode(
     scale = softmax_scale if softmax_scale is not None else 1.0 / math.sqrt(plan.head_dim)
     with _paged.current(device):
         stream = _paged.current_stream(device)
+        if found:
+            _paged.keep_for_graphs(plan)
         tables = plan.device_tables(device, stream)
         # (the plain decode may split long requests through scratch that belongs to the stream, which graphs that
         # were captured on it would share; a captured call does without)
