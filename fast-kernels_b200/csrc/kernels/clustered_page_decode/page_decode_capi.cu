@@ -337,15 +337,15 @@ int variant_shared_bytes(const Variant& v, int warps, int stages) {
   return -1;
 }
 
-cudaError_t launch_variant(const Variant& v, const DecodeParams& params, int blocks, int warps, int stages,
+cudaError_t launch_variant(const Variant& v, const JoinedDecodeParams& params, int blocks, int warps, int stages,
                            cudaStream_t stream) {
   if (v.tensor_cores) {
-#define FK_PD_LAUNCH_MMA(NAME) launch_mma_##NAME(params, blocks, warps, stages, stream)
+#define FK_PD_LAUNCH_MMA(NAME) launch_mma_##NAME(v.joined, params, blocks, warps, stages, stream)
     FK_PD_DISPATCH(FK_PD_LAUNCH_MMA)
 #undef FK_PD_LAUNCH_MMA
     return cudaErrorInvalidValue;
   }
-#define FK_PD_LAUNCH(NAME) launch_##NAME(v.keys_are_rotated, v.group_tile, params, blocks, warps, stages, stream)
+#define FK_PD_LAUNCH(NAME) launch_##NAME(v.keys_are_rotated, v.group_tile, v.joined, params, blocks, warps, stages, stream)
   FK_PD_DISPATCH(FK_PD_LAUNCH)
 #undef FK_PD_LAUNCH
   return cudaErrorInvalidValue;
@@ -370,7 +370,7 @@ int forward(const fk_page_decode_args* args, const fk_page_decode_prior* prior) 
   if (const int code = device_info(&info); code != FK_PAGE_DECODE_OK) {
     return code;
   }
-  DecodeParams params{};
+  JoinedDecodeParams params{};
   params.query = static_cast<const uint16_t*>(a.query);
   params.key_pages = static_cast<const uint8_t*>(a.key_pages);
   params.value_pages = static_cast<const uint8_t*>(a.value_pages);
@@ -394,6 +394,7 @@ int forward(const fk_page_decode_args* args, const fk_page_decode_prior* prior) 
   params.head_tiles = plan.head_tiles;
   params.page_size = a.page_size;
   if (prior != nullptr) {
+    plan.variant.joined = true;
     params.prior = prior->rows;
     params.prior_of_request = reinterpret_cast<const int2*>(prior->of_request);
   }
