@@ -23,8 +23,8 @@ def test_the_plain_instances_have_nothing_of_the_join() -> None:
             uses += 1
             assert any(open_blocks), line
         for brace in re.findall(r"if constexpr \(JOIN\) \{|[{}]", line):
-            if brace == "}":
-                open_blocks.pop()
-            else:
+            if brace != "}":
                 open_blocks.append(brace != "{")
+            elif open_blocks:  # (the namespace's own brace closes last)
+                open_blocks.pop()
     assert uses >= 3
