@@ -36,12 +36,18 @@ __device__ __forceinline__ void share_rope_table(const RopeTable& table, uint64_
     }
   }
 }
+// The nearest quarter turn comes off in integers, so that what is left, at most an eighth of a turn, loses no more than
+// 2^-28 of a turn to fp32: an error of 2.3e-8 at most. (Rounding the whole angle loses up to 9.4e-8, rms twice that of an
+// fp32 cosine; a correction behind the cosine is lost in its rounding.)
 __device__ __forceinline__ float2 rope_cos_sin(uint64_t turns_per_position, int position) {
-  const uint64_t turns = turns_per_position * static_cast<uint32_t>(position);
-  const float half_turns = static_cast<float>(static_cast<int32_t>(turns >> 32)) * 0x1p-31f;  // in [-1, 1]
+  const uint32_t turns = static_cast<uint32_t>((turns_per_position * static_cast<uint32_t>(position)) >> 32);
+  const uint32_t quarters = (turns + 0x20000000u) >> 30;
+  const float half_turns = static_cast<float>(static_cast<int32_t>(turns - (quarters << 30))) * 0x1p-31f;  // in [-1/4, 1/4]
   float sn, cs;
   sincospif(half_turns, &sn, &cs);
-  return make_float2(cs, sn);
+  const float c = (quarters & 1u) != 0 ? -sn : cs;
+  const float s = (quarters & 1u) != 0 ? cs : sn;
+  return (quarters & 2u) != 0 ? make_float2(-c, -s) : make_float2(c, s);
 }
 
 // The same, off by up to 2^-20.5: for a query that is rounded to 16 bits behind it.

@@ -1,0 +1,62 @@
+"""The rotary angles of the paged-cache operators."""
+
+from __future__ import annotations
+
+import importlib
+import math
+from decimal import Decimal, getcontext
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+ops = importlib.import_module("fast_kernels.ops")
+
+
+def _angles(positions: np.ndarray, dim: int, theta: float) -> tuple[np.ndarray, np.ndarray]:
+    """[positions, pairs]: position * theta^(-2i/dim) in radians, the whole turns taken off in exact arithmetic; and what
+    rounding half an angle's turns to fp32 leaves out of it."""
+    getcontext().prec = 60
+    pi = Decimal("3.14159265358979323846264338327950288419716939937510582097494459")
+    per_position = [int((Decimal(theta).ln() * Decimal(-2 * i) / dim).exp() / (2 * pi) * 2**64) for i in range(dim // 2)]
+    upper = np.array([[((int(p) * t) % 2**64) >> 32 for t in per_position] for p in positions], dtype=np.int64)
+    upper = np.where(upper >= 2**31, upper - 2**32, upper)
+    rest = upper - upper.astype(np.float32).astype(np.int64)
+    return upper * (math.pi / 2**31), rest * (math.pi / 2**31)
+
+
+def test_an_appended_keys_angle_is_not_rounded_to_fp32() -> None:
+    """Every key has a single element of 1, which its turn makes (cos, sin): the page's scale times 127 is the larger of the
+    two. It is off by at most 2^-24 (an fp32 cosine within one unit in the last place, below 1) and 2^-24 (the quotient), and
+    these have nothing to do with the sign of what rounding the whole angle leaves out: over N keys the mean of the errors,
+    each times that sign, stays within 6 * 2^-23 / sqrt(N), 2.8e-9. With the angle rounded the mean is its share of the error,
+    about 3e-8 * 0.35.
+
+    What rounding the angle's distance to a quarter turn leaves out (in units u = pi * 2^-31: w(rest), rest brought into +-16
+    or less) has no part in the mean where the whole angle's rounding is coarser: w is as often up as down over +-32 or +-64.
+    Where it is the same rounding, in the eighth of the turn around 0, its mean is 8 u on |angle| in [1/16, 1/8] of a turn, half
+    of that in the interval of half the length before, and so on: 8 u * 1/8 * (1 + 1/4 + 1/16 + ..) * the slope's 0.71 < 1.4e-9."""
+    heads, dim, ps, tokens, theta = 32, 64, 16, 2048, 10000.0
+    positions = np.random.RandomState(1).randint(0, 100_000 // ps, tokens) * ps
+    table = np.full((tokens, 100_000 // ps + 1), -1, dtype=np.int32)
+    table[np.arange(tokens), positions // ps] = np.arange(tokens)
+    lens = torch.from_numpy(positions.astype(np.int32))
+    cache = ops.empty_paged_kv(num_pages=tokens, page_table=torch.from_numpy(table), seq_lens=lens, num_kv_heads=heads, head_dim=dim,
+                               page_size=ps, kv_layout="int8_kv", key_rope_theta=theta)
+    keys = torch.zeros((tokens, heads, dim), dtype=torch.bfloat16, device="cuda")
+    pair = torch.arange(heads, device="cuda")
+    keys[:, pair, 2 * pair] = 1.0
+    plan = ops.plan_paged_kv_append(page_table=cache.page_table, seq_lens=lens, append_lens=torch.ones(tokens, dtype=torch.int32),
+                                    num_kv_heads=heads, head_dim=dim, page_size=ps, kv_layout="int8_kv", use_cache=False)
+    ops.paged_kv_append(keys, keys, cache, plan=plan)
+    got = cache.key_scales[:, :, 0].double().cpu().numpy() * 127.0
+    angle, rest = _angles(positions, dim, theta)
+    cos, sin = np.cos(angle), np.sin(angle)
+    of_cos = np.abs(cos) >= np.abs(sin)
+    want = np.where(of_cos, np.abs(cos), np.abs(sin))
+    slope = np.where(of_cos, -sin * np.sign(cos), cos * np.sign(sin))
+    off = got - want
+    assert np.abs(off).max() <= 2.0**-23
+    mean = float((off * np.sign(-rest * slope)).mean())
+    assert abs(mean) <= 6 * 2.0**-23 / math.sqrt(off.size), mean
