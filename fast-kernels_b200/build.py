@@ -80,7 +80,8 @@ def build_page_decode_library(force: bool = False) -> Path:
     kernel_dir = CSRC / "kernels" / "clustered_page_decode"
     sources = sorted(kernel_dir.glob("*.cu"))
     deps = (sources + sorted(kernel_dir.glob("*.cuh")) + sorted(kernel_dir.glob("*.h")) + sorted(kernel_dir.glob("*.inc"))
-            + [REPO / "include" / "fk_page_decode.h", CSRC / "kernels" / "decode_quant_linear" / "w4a16_common.cuh"])
+            + [REPO / "include" / "fk_page_decode.h", CSRC / "kernels" / "decode_quant_linear" / "w4a16_common.cuh",
+               CSRC / "kernels" / "paged_kv" / "rope_turns.cuh"])
     target = LIB_DIR / "libfk_page_decode.so"
     if not force and _newer(target, deps):
         return target

@@ -186,6 +186,7 @@ int make_plan(const fk_page_decode_args& a, Plan* plan, bool check_workspace = t
     tile = 4;
   }
   out.variant = Variant{a.head_dim, a.kv_format, a.keys_are_rotated != 0, tile};
+  out.variant.joined = merged;
   if (tensor_cores_enabled() && a.keys_are_rotated != 0) {
     // keys that carry their rotation are exact tensor-core operands (8-bit elements convert to
     // bf16 exactly): logits and weighted values as mma.sync, always with the full tile of 8 heads
@@ -326,12 +327,12 @@ int make_plan(const fk_page_decode_args& a, Plan* plan, bool check_workspace = t
 
 int variant_shared_bytes(const Variant& v, int warps, int stages) {
   if (v.tensor_cores) {
-#define FK_PD_SHARED_MMA(NAME) shared_bytes_mma_##NAME(warps, stages)
+#define FK_PD_SHARED_MMA(NAME) shared_bytes_mma_##NAME(v.joined, warps, stages)
     FK_PD_DISPATCH(FK_PD_SHARED_MMA)
 #undef FK_PD_SHARED_MMA
     return -1;
   }
-#define FK_PD_SHARED(NAME) shared_bytes_##NAME(v.keys_are_rotated, v.group_tile, warps, stages)
+#define FK_PD_SHARED(NAME) shared_bytes_##NAME(v.keys_are_rotated, v.group_tile, v.joined, warps, stages)
   FK_PD_DISPATCH(FK_PD_SHARED)
 #undef FK_PD_SHARED
   return -1;
@@ -394,9 +395,9 @@ int forward(const fk_page_decode_args* args, const fk_page_decode_prior* prior) 
   params.head_tiles = plan.head_tiles;
   params.page_size = a.page_size;
   if (prior != nullptr) {
-    plan.variant.joined = true;
     params.prior = prior->rows;
     params.prior_of_request = reinterpret_cast<const int2*>(prior->of_request);
+    fk_rope::fill_rope_table(&params.rope, a.head_dim, a.rope_theta);
   }
   params.splits = plan.splits;
   params.stages = plan.stages;

@@ -38,6 +38,7 @@
 #include <type_traits>
 
 #include "../decode_quant_linear/w4a16_common.cuh"
+#include "../paged_kv/rope_turns.cuh"
 #include "page_decode_mma.cuh"
 
 namespace fk_page_decode {
@@ -105,12 +106,16 @@ struct JoinedDecodeParams : DecodeParams {
   // for it comes last. NULL: none.
   const float* prior;
   const int2* prior_of_request;
+  // Queries that meet keys with their rotation in them are turned by these angles instead of the fp32 product
+  // position * inv_freq: whoever made the prior rows turned the same query by them, and the keys
+  // (paged_kv_append) were. The product is off by 3e-3 radians at position 131071, 5e-2 at 1000000.
+  fk_rope::RopeTable rope;
 };
 
 __host__ __device__ constexpr int round_up(int v, int m) { return (v + m - 1) / m * m; }
 
 // Shared-memory layout, the same arithmetic on host (size) and device (offsets).
-template <int D, int KV, bool ROT, int GT, bool MMA = false>
+template <int D, int KV, bool ROT, int GT, bool MMA = false, bool JOIN = false>
 struct Layout {
   static constexpr int kElemBytes = KV == kKvBf16 ? 2 : 1;
   static constexpr bool kQuant = KV != kKvBf16;
@@ -130,6 +135,8 @@ struct Layout {
   // run-time alignment of the shared-memory address; kAlign bytes of slack pay for it.
   static constexpr int kAlign = ROT ? kUnitBytes : (kRopeBytes > kUnitBytes ? kRopeBytes : kUnitBytes);
   static constexpr int kEpl = D / 32;
+  static constexpr bool kTurns = ROT && JOIN;  // 64-bit turns per position in the place of inv_freq
+  static constexpr int kInvFreqBytes = kTurns && D / 2 * 8 > kMaxPairs * 4 ? D / 2 * 8 : kMaxPairs * 4;
 
   int bars, entries, kscales, inv_freq, vscales, probs, alphas, converted, tail, total;
 
@@ -142,7 +149,7 @@ struct Layout {
     kscales = at;
     at += kQuant ? kEntryCapacity * kDimBlocks * 4 : 0;
     inv_freq = at;
-    at += kMaxPairs * 4;
+    at += kInvFreqBytes;
     vscales = at;
     at += round_up(warps * stages * kVScaleBytes, 128);
     probs = at;
@@ -343,7 +350,7 @@ template <int D, int KV, bool ROT, int GT, bool MMA = false, bool JOIN = false>
 __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 32, 1)
     page_decode_kernel(const __grid_constant__ std::conditional_t<JOIN, JoinedDecodeParams, DecodeParams> p) {
   static_assert(!MMA || (ROT && GT == 8), "the tensor-core variant: rotated keys, tiles of 8");
-  using L = Layout<D, KV, ROT, GT, MMA>;
+  using L = Layout<D, KV, ROT, GT, MMA, JOIN>;
   constexpr bool PAIRS = L::kPairStage;  // the stage itself holds skewed row pairs (bf16 pages on tensor cores)
   constexpr int EPL = L::kEpl;
   constexpr int EB = L::kElemBytes;
@@ -406,9 +413,23 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
   for (int i = tid; i < warps * stages; i += threads) {
     mbar_init(bars + i * 8, 1);
   }
+  [[maybe_unused]] uint64_t* turns_s = reinterpret_cast<uint64_t*>(smem + layout.inv_freq);
   for (int i = tid; i < D / 2; i += threads) {  // a block may have fewer threads than pairs
-    inv_freq_s[i] = p.inv_freq[i];
+    if constexpr (L::kTurns) {
+      turns_s[i] = p.rope.turns[i];
+    } else {
+      inv_freq_s[i] = p.inv_freq[i];
+    }
   }
+  auto query_turn = [&](int position, int pair, float* cs, float* sn) {
+    if constexpr (L::kTurns) {
+      const float2 turn = fk_rope::rope_cos_sin(turns_s[pair], position);
+      *cs = turn.x;
+      *sn = turn.y;
+    } else {
+      sincosf(static_cast<float>(position) * inv_freq_s[pair], sn, cs);
+    }
+  };
   mbar_init_fence();
   // Programmatic dependent launch (no-ops without the launch attribute): the next kernel of the
   // stream may be scheduled from here on. What follows up to the wait touches no global memory:
@@ -601,7 +622,7 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
     if (round == 0 && MMA) {
       const int head = lane >> 2;
       tensor.prepare(head < tile_heads ? p.query + out_base + static_cast<size_t>(head) * D : nullptr, lane,
-                     query_position, inv_freq_s, p.scale_log2e, reinterpret_cast<float*>(probs),
+                     query_position, query_turn, p.scale_log2e, reinterpret_cast<float*>(probs),
                      kShiftKeys ? 256.0f : 1.0f, kShiftValues ? 256.0f : 1.0f);
     }
     if (round == 0 && !MMA) {
@@ -623,9 +644,11 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
       }
 #pragma unroll
       for (int i = 0; i < EPL / 2; ++i) {
-        inv_freq_lane[i] = inv_freq_s[lane * (EPL / 2) + i];
+        if constexpr (!L::kTurns) {
+          inv_freq_lane[i] = inv_freq_s[lane * (EPL / 2) + i];
+        }
         if constexpr (ROT) {
-          sincosf(static_cast<float>(query_position) * inv_freq_lane[i], &rot_sin[i], &rot_cos[i]);
+          query_turn(query_position, lane * (EPL / 2) + i, &rot_cos[i], &rot_sin[i]);
         } else {
           sincosf(static_cast<float>(-U * unit_step) * inv_freq_lane[i], &step_sin[i], &step_cos[i]);
         }

@@ -24,7 +24,7 @@ cudaError_t launch_variant(const Variant& v, const JoinedDecodeParams& params, i
                            cudaStream_t stream);
 
 #define FK_PAGE_DECODE_DECLARE_SHAPE(NAME)                                                              \
-  int shared_bytes_##NAME(bool rotated, int group_tile, int warps, int stages);                        \
+  int shared_bytes_##NAME(bool rotated, int group_tile, bool joined, int warps, int stages);           \
   cudaError_t launch_##NAME(bool rotated, int group_tile, bool joined, const JoinedDecodeParams& params, \
                             int blocks, int warps, int stages, cudaStream_t stream);
 FK_PAGE_DECODE_DECLARE_SHAPE(d64_bf16)
@@ -35,7 +35,7 @@ FK_PAGE_DECODE_DECLARE_SHAPE(d128_fp8)
 FK_PAGE_DECODE_DECLARE_SHAPE(d128_int8)
 #undef FK_PAGE_DECODE_DECLARE_SHAPE
 #define FK_PAGE_DECODE_DECLARE_MMA(NAME)                            \
-  int shared_bytes_mma_##NAME(int warps, int stages);               \
+  int shared_bytes_mma_##NAME(bool joined, int warps, int stages);  \
   cudaError_t launch_mma_##NAME(bool joined, const JoinedDecodeParams& params, int blocks, int warps, int stages, \
                                 cudaStream_t stream);
 FK_PAGE_DECODE_DECLARE_MMA(d64_bf16)

@@ -122,11 +122,13 @@ struct MmaWarp {
   float o_power;          // HALF: a fixed power of two `o` is divided by on top of that
 
   // `query_row` -> bf16 query of head g (nullptr for a row past the tile); rotated by
-  // position * theta, scaled by `scale`. `scratch`: D floats of this warp's shared memory, used to
-  // hand the D/2 (cos, sin) pairs -- two sincosf per lane -- to the lanes that need them.
+  // position * theta -- turn(position, pair, &cos, &sin) --, scaled by `scale`. `scratch`: D floats of this
+  // warp's shared memory, used to hand the D/2 (cos, sin) pairs -- two turns per lane -- to the lanes that need
+  // them.
   // HALF: the key rows hold the keys divided by `key_power`, the value rows the values divided by
   // `value_power` (powers of two).
-  __device__ __forceinline__ void prepare(const uint16_t* query_row, int lane, int position, const float* inv_freq,
+  template <class Turn>
+  __device__ __forceinline__ void prepare(const uint16_t* query_row, int lane, int position, const Turn& turn,
                                           float scale, float* scratch, float key_power = 1.0f,
                                           float value_power = 1.0f) {
     o_power = value_power;
@@ -139,7 +141,7 @@ struct MmaWarp {
     l_run = 0.0f;
     for (int pair = lane; pair < D / 2; pair += 32) {
       float sn, cs;
-      sincosf(static_cast<float>(position) * inv_freq[pair], &sn, &cs);
+      turn(position, pair, &cs, &sn);
       *reinterpret_cast<float2*>(scratch + 2 * pair) = make_float2(cs * scale, sn * scale);
     }
     __syncwarp();

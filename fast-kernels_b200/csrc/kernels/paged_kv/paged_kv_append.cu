@@ -45,26 +45,6 @@ int fail_cuda(const char* what, cudaError_t err) {
   return fail(FK_PAGED_KV_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(err));
 }
 
-void fill_rope_table(RopeTable* table, int head_dim, float theta) {
-  // 64 powers take longer than the rest of a call; a thread's calls have the same ones nearly always
-  thread_local RopeTable kept;
-  thread_local int kept_dim = 0;
-  thread_local float kept_theta = 0.0f;
-  if (kept_dim != head_dim || kept_theta != theta) {
-    for (int i = 0; i < head_dim / 2; ++i) {
-      // long double: 64 bits of mantissa, so that far positions lose nothing (a theta below 1 turns pairs by
-      // more than a turn per position; the whole turns do not matter)
-      const long double turns = std::pow(static_cast<long double>(theta), -2.0L * i / head_dim) / 6.283185307179586476925286766559L;
-      const long double fraction = turns - std::floor(turns);
-      const long double scaled = std::round(fraction * 18446744073709551616.0L);
-      kept.turns[i] = scaled >= 18446744073709551616.0L ? 0 : static_cast<uint64_t>(scaled);
-    }
-    kept_dim = head_dim;
-    kept_theta = theta;
-  }
-  *table = kept;
-}
-
 }  // namespace fk_paged_kv
 
 using namespace fk_paged_kv;

@@ -128,7 +128,9 @@ FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args);
  * them already (fk_paged_kv_attention): request b's result is merged with prior rows
  *     rows[(of_request[b][0] + j) * num_q_heads + q_head],  j < of_request[b][1]
  * of head_dim + 4 floats (weighted values, maximum of the logits in units of ln 2, denominator, two
- * unused). A request may have prior rows and no runs. seq_lens still says where the query sits. The
+ * unused). A request may have prior rows and no runs. seq_lens still says where the query sits; with
+ * keys_are_rotated the query is turned by the angle that fk_paged_kv_attention turns it by (64-bit fixed point)
+ * instead of the fp32 product position * frequency of fk_page_decode_forward. The
  * kernel launched before this one on the stream must be the one that writes the rows; it may write
  * nothing else that this call reads, and must itself have waited for the kernel before it. */
 typedef struct fk_page_decode_prior {

@@ -9,6 +9,8 @@ from decimal import Decimal, getcontext
 import numpy as np
 import pytest
 import torch
+from fast_kernels.native import native_module
+from paged_kv_testlib import cache_values, random_cache, rotate64
 
 pytestmark = pytest.mark.gpu
 ops = importlib.import_module("fast_kernels.ops")
@@ -60,3 +62,46 @@ def test_an_appended_keys_angle_is_not_rounded_to_fp32() -> None:
     assert np.abs(off).max() <= 2.0**-23
     mean = float((off * np.sign(-rest * slope)).mean())
     assert abs(mean) <= 6 * 2.0**-23 / math.sqrt(off.size), mean
+
+
+@pytest.mark.parametrize("layout", ["bf16_kv", "fp8_kv", "int8_kv"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_shared_decode_far_out_turns_its_queries_by_one_angle(layout, dim) -> None:
+    """Two requests share a million tokens, one page over and over, whose keys are 0: logits of 0, whatever the angle. Their
+    own last tokens have logits to about +-40, and nearly all of the weight.
+
+    Of these the query is a 16-bit head and remainder (2^-17 with bf16) and its turn fp32: d = 2^-16 * scale * max_t sum_i
+    |q_i k_i| on a logit, a factor within e^(+-2 d) on a weight; 16-bit heads and remainders of the weights: 2^-16. The shared part's
+    weights are rounded to bf16 or fp16, and 8-bit values of the block without the token's larger scale to fp16 twice: 2^-8 of
+    its sum. The row is rounded once. An fp32 angle is off by up to 0.05 here."""
+    ps, theta, shared, own = 32, 10000.0, 31_250, 25
+    table = np.zeros((2, shared + 1), dtype=np.int32)
+    table[:, -1] = [1, 2]
+    length = shared * ps + own
+    cache = random_cache(layout=layout, pages=3, heads=2, page_size=ps, dim=dim, table=table, lens=[length, length - 8], theta=theta, seed=1)
+    cache.key_pages[0] = 0
+    query = torch.randn((2, 8, dim), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    plan = ops.plan_shared_prefix_decode(page_table=cache.page_table, seq_lens=cache.seq_lens, num_q_heads=8, num_kv_heads=2, head_dim=dim,
+                                         page_size=ps, kv_layout=layout, min_saved_bytes=0, use_cache=False)
+    assert plan.runs == [(0, shared, (0, 1))]
+    scale = 8.0 / math.sqrt(dim)
+    got = ops.shared_prefix_decode(query, cache, plan=plan, softmax_scale=scale).double().cpu()
+    keys, values = cache_values(cache)
+    for b, n in enumerate(cache.seq_lens.tolist()):
+        turned = rotate64(query[b : b + 1].cpu(), [n - 1], theta)[0].reshape(2, 4, dim)
+        k, v = keys[1 + b, :, : n - shared * ps], values[1 + b, :, : n - shared * ps]
+        logits = torch.einsum("hgd,htd->hgt", turned, k) * scale
+        top = logits.amax(dim=-1, keepdim=True)
+        weights, before = torch.exp(logits - top), torch.exp(-top) * shared
+        total = weights.sum(dim=-1, keepdim=True) + before * ps
+        mine = torch.einsum("hgt,htd->hgd", weights, v) / total
+        others = before * values[0].sum(dim=1)[:, None] / total
+        want = mine + others
+        d = 2.0**-16 * scale * torch.einsum("hgd,htd->hgt", turned.abs(), k.abs()).amax(dim=-1, keepdim=True)
+        a_mine = torch.einsum("hgt,htd->hgd", weights, v.abs()) / total
+        a_others = before * values[0].abs().sum(dim=1)[:, None] / total
+        bound = 2.0**-8 * want.abs() + (2.0**-16 + 2.2 * d) * (a_mine + a_others) + 2.0**-8 * a_others
+        off = (got[b].reshape(2, 4, dim) - want).abs()
+        assert float((off / bound).max()) <= 1.0, float((off / bound).max())
+    torch.cuda.synchronize()
+    assert native_module().paged_kv_device_status() == 0 and native_module().page_decode_device_status() == 0
