@@ -444,6 +444,18 @@ FK_PAGE_DECODE_API int fk_page_decode_workspace_init(void* workspace, size_t wor
   return err == cudaSuccess ? FK_PAGE_DECODE_OK : fail_cuda("cudaMemsetAsync", err);
 }
 
+FK_PAGE_DECODE_API int fk_page_decode_workspace_need(const fk_page_decode_args* args, size_t* bytes) {
+  if (args == nullptr || bytes == nullptr) {
+    return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "workspace_need: args and bytes must not be NULL");
+  }
+  Plan plan;
+  if (const int code = make_plan(*args, &plan, false); code != FK_PAGE_DECODE_OK) {
+    return code;
+  }
+  *bytes = plan.workspace_need;
+  return FK_PAGE_DECODE_OK;
+}
+
 FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args) { return forward(args, nullptr); }
 
 FK_PAGE_DECODE_API int fk_page_decode_forward_merged(const fk_page_decode_args* args, const fk_page_decode_prior* prior) {

@@ -16,9 +16,10 @@ void clustered_page_decode_forward(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, 
   unavailable();
 }
 void clustered_page_decode_forward_hinted(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, int, int, int, int,
-                                          int, int, int, int, int, int, int, float, float, int, int, ptr) {
+                                          int, int, int, int, int, int, int, float, float, int, int, ptr, ptr) {
   unavailable();
 }
+std::size_t page_decode_workspace_bytes(int, int, int, int) { unavailable(); }
 int page_decode_device_status() { unavailable(); }
 
 }  // namespace fast_kernels::clustered_page_decode

@@ -106,7 +106,7 @@ void shared_prefix_decode_forward(
     std::uintptr_t partials_ptr, int batch, int num_page_ids, int num_items, int num_partials, int num_runs,
     int max_tail_pages, int num_pages, int num_q_heads, int num_kv_heads, int head_dim, int page_size, int kv_format,
     float softmax_scale, float rope_theta, std::uintptr_t stream_ptr) {
-  if (num_items < 0 || (num_items > 0) != (num_partials > 0)) {
+  if (num_items <= 0 || num_partials <= 0) {
     throw std::invalid_argument("shared_prefix_decode: items and partial results come together");
   }
   fk_page_decode_args tail{};
@@ -172,14 +172,9 @@ void shared_prefix_decode_forward(
   args.softmax_scale = softmax_scale;
   args.rope_theta = rope_theta;
   args.stream = tail.stream;
-  int code = FK_PAGE_DECODE_OK;
-  if (num_items > 0) {
-    raise_if_failed(fk_paged_kv_attention(&args));
-    fk_page_decode_prior prior{as<const float>(partials_ptr), as<const int32_t>(of_request_ptr)};
-    code = fk_page_decode_forward_merged(&tail, &prior);
-  } else {
-    code = fk_page_decode_forward(&tail);
-  }
+  raise_if_failed(fk_paged_kv_attention(&args));
+  const fk_page_decode_prior prior{as<const float>(partials_ptr), as<const int32_t>(of_request_ptr)};
+  const int code = fk_page_decode_forward_merged(&tail, &prior);
   if (code == FK_PAGE_DECODE_ERR_INVALID_ARGUMENT) {
     throw std::invalid_argument(fk_page_decode_last_error());
   }

@@ -24,8 +24,8 @@ void paged_attention_forward(
     float rope_theta, std::uintptr_t stream_ptr);
 
 // Decode behind shared runs of pages: the runs' items (fk_paged_kv_attention), then every request's own
-// tokens merged with them (fk_page_decode_forward_merged); without items the plain decode. Uses no scratch
-// of this layer's own: calls on several streams, and captured ones, do not share any.
+// tokens merged with them (fk_page_decode_forward_merged). Uses no scratch of this layer's own: calls on several
+// streams, and captured ones, do not share any.
 void shared_prefix_decode_forward(
     std::uintptr_t query_ptr, std::uintptr_t key_ptr, std::uintptr_t value_ptr, std::uintptr_t key_scales_ptr,
     std::uintptr_t value_scales_ptr, std::uintptr_t page_ids_ptr, std::uintptr_t vectors_ptr, std::uintptr_t items_ptr,

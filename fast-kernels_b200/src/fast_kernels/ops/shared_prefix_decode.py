@@ -34,14 +34,17 @@ from fast_kernels.ops.clustered_page_decode import (
     PagedKVCache,
     _layout_id,
     _torch,
-    clustered_page_decode,
     plan_clustered_page_decode,
 )
 from fast_kernels.ops.prefix_union_decode import _shared_page_bytes
 
 _PLANS: OrderedDict = OrderedDict()
-# Bytes that a plan has to save before it shares. Measured with 8 kv heads of 128, us with sharing / without: bf16, 62 MB
-# saved 24.5 / 20.5, 124 MB 24.6 / 26.7, 248 MB 26.7 / 41.1; int8, 32 MB 28.6 / 22.6, 64 MB 28.7 / 30.9, 128 MB 32.8 / 49.4.
+# Bytes that a plan has to save before it shares. Measured in graphs, us with sharing / without, requests with 200 tokens of
+# their own behind 1024 that they share. 8 kv heads of 128 x 4 query heads, bf16: 63 MB saved 21.9 / 19.1, 130 MB 25.5 / 27.2,
+# 264 MB 35.8 / 51.9; int8: 32 MB 26.4 / 21.4, 67 MB 29.7 / 31.7, 136 MB 40.8 / 59.5. 8 heads of 64 x 2, bf16: 31 MB
+# 18.7 / 15.7, 65 MB 19.9 / 22.6; int8: 34 MB 23.0 / 21.8, 68 MB 26.2 / 40.4. 32 heads of 128 x 1, bf16: 117 MB 26.3 / 26.3,
+# 252 MB 33.2 / 49.9. Not the bytes alone count: 4096 shared tokens pay from 25 to 60 MB on, and few heads with many
+# requests later (2 heads of 128 x 8, 64 requests, bf16: 66 MB 26.0 / 20.1).
 DEFAULT_MIN_SAVED_BYTES = 64 << 20
 # Shared runs shorter than this stay with the requests (or with longer runs further down).
 MIN_RUN_TOKENS = 128
@@ -246,15 +249,24 @@ def shared_prefix_decode(
         if found:
             _paged.keep_for_graphs(plan)
         tables = plan.device_tables(device, stream)
-        # (the plain decode may split long requests through scratch that belongs to the stream, which graphs that
-        # were captured on it would share; a captured call does without)
-        if not plan.runs and not torch.cuda.is_current_stream_capturing():
-            return clustered_page_decode(query, cache, plan=plan.tail_plan, output=output, softmax_scale=scale,
-                                         rope_theta=rope_theta)
-        partials = None
-        if plan.runs:
-            partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
         tail = plan.tail_plan
+        if not plan.runs:  # the launch that clustered_page_decode makes
+            # (it may split long requests through scratch: the stream's, or, since graphs that were captured on one stream
+            # may be replayed at the same time, a captured call's own)
+            scratch = None
+            if torch.cuda.is_current_stream_capturing():
+                scratch = torch.empty(native.page_decode_workspace_bytes(plan.batch, plan.num_q_heads, plan.num_kv_heads, plan.head_dim),
+                                      dtype=torch.uint8, device=device)
+            direct = tail.launch_mode == "direct"
+            native.clustered_page_decode_forward(
+                query.data_ptr(), cache.key_pages.data_ptr(), cache.value_pages.data_ptr(), _paged.address(cache.key_scales),
+                _paged.address(cache.value_scales), tables["run_base_pages"], tables["run_page_counts"], tables["run_logical_starts"],
+                tables["run_last_page_lens"], tables["request_run_offsets"], tables["seq_lens"], output.data_ptr(), plan.batch,
+                tail.num_runs, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, plan.page_size, tail.group_tile, int(not direct),
+                1 if direct else max(2, tail.cluster_size), _layout_id(plan.kv_layout), int(cache.keys_are_rotated), float(scale),
+                float(rope_theta), stream, max_pages_hint=tail.max_pages, early_descriptors=1, workspace_ptr=_paged.address(scratch))
+            return output
+        partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
         native.shared_prefix_decode_forward(
             query.data_ptr(), cache.key_pages.data_ptr(), cache.value_pages.data_ptr(), _paged.address(cache.key_scales),
             _paged.address(cache.value_scales), tables["page_ids"], tables["vectors"], tables["items"], tables["of_request"],

@@ -75,6 +75,7 @@ SIGNATURES = {
     "fk_page_decode_last_error": (ctypes.c_char_p, []),
     "fk_page_decode_workspace_bytes": (_c_size_t, [ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int]),
     "fk_page_decode_workspace_init": (ctypes.c_int, [_c_void_p, _c_size_t, _c_void_p]),
+    "fk_page_decode_workspace_need": (ctypes.c_int, [ctypes.POINTER(PageDecodeArgs), ctypes.POINTER(_c_size_t)]),
     "fk_page_decode_forward": (ctypes.c_int, [ctypes.POINTER(PageDecodeArgs)]),
     "fk_page_decode_forward_merged": (ctypes.c_int, [ctypes.POINTER(PageDecodeArgs), ctypes.POINTER(PageDecodePrior)]),
     "fk_page_decode_device_status": (ctypes.c_int, [ctypes.POINTER(ctypes.c_int)]),

@@ -120,6 +120,9 @@ FK_PAGE_DECODE_API const char* fk_page_decode_last_error(void);
 FK_PAGE_DECODE_API size_t fk_page_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads,
                                                          int head_dim);
 FK_PAGE_DECODE_API int fk_page_decode_workspace_init(void* workspace, size_t workspace_bytes, void* stream);
+/* How much of its workspace a call with these arguments uses: 0 if it is not split, or merges through shared
+ * memory, and then the workspace need not be initialised for it. */
+FK_PAGE_DECODE_API int fk_page_decode_workspace_need(const fk_page_decode_args* args, size_t* bytes);
 
 /* Replaces clustered_page_decode_forward (clustered_page_decode.h:16-25). */
 FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args);

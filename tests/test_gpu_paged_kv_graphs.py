@@ -60,3 +60,44 @@ def test_a_graph_outlives_the_memory_of_the_plans_that_its_calls_found() -> None
     assert all(_same_bits(a, b) for a, b in zip(got, want))
     del rubbish
     _status_ok()
+
+
+def test_without_sharing_captured_calls_are_the_eager_one_with_scratch_of_their_own() -> None:
+    """Two long requests on few heads: split over as many blocks as the device has room for, through scratch. The same
+    bits as the plain decode, eager and from two graphs that replay side by side on queries of their own."""
+    table, pages = fragmented_table([500, 450], 1)
+    cache = random_cache(layout="bf16_kv", pages=pages, heads=2, page_size=32, dim=128, table=table, lens=[15_990, 14_400], theta=10000.0, seed=2)
+    plan = ops.plan_shared_prefix_decode(page_table=cache.page_table, seq_lens=cache.seq_lens, num_q_heads=8, num_kv_heads=2, head_dim=128,
+                                         page_size=32, kv_layout="bf16_kv", use_cache=False)
+    assert plan.runs == []
+    queries = [_rows(2, 8, 128, seed) for seed in (3, 4)]
+    wants = [ops.clustered_page_decode(query, cache) for query in queries]
+    for query, want in zip(queries, wants):
+        assert _same_bits(ops.shared_prefix_decode(query, cache, plan=plan), want)
+    torch.cuda.synchronize()
+    graphs, side = [], torch.cuda.Stream()
+    for query in queries:
+        graph, output = torch.cuda.CUDAGraph(), torch.empty_like(query)
+        with torch.cuda.graph(graph, stream=side):
+            ops.shared_prefix_decode(query, cache, plan=plan, output=output)
+        graphs.append((graph, output))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(20):
+        for stream, (graph, output) in zip(streams, graphs):
+            with torch.cuda.stream(stream):
+                output.zero_()
+                graph.replay()
+    torch.cuda.synchronize()
+    for (_, output), want in zip(graphs, wants):
+        assert _same_bits(output, want)
+    _status_ok()
+
+
+def test_without_sharing_large_head_groups_and_short_requests_are_the_plain_decode() -> None:
+    for group, lens in ((12, [40, 3]), (60, [33, 700]), (3, [1, 0])):
+        counts = [-(-n // 16) for n in lens]
+        table, pages = fragmented_table(counts, 1)
+        cache = random_cache(layout="int8_kv", pages=pages, heads=2, page_size=16, dim=64, table=table, lens=lens, theta=10000.0, seed=2)
+        query = _rows(2, 2 * group, 64, 3)
+        assert _same_bits(ops.shared_prefix_decode(query, cache), ops.clustered_page_decode(query, cache))
+    _status_ok()
