@@ -240,7 +240,16 @@ int make_plan(const fk_page_decode_args& a, Plan* plan, bool check_workspace = t
   }
 
   int splits = a.splits;
-  if (splits == 0) {
+  if (splits == 0 && merged && a.workspace == nullptr) {
+    // Without scratch: one block per task, or a cluster of 2 or 4 that merges through shared memory, where
+    // there are few tasks and each block still has two rounds of 8 warps to do.
+    const long long units = static_cast<long long>(a.max_pages_hint) * (a.page_size / kUnitTokens);
+    splits = 1;
+    while (cluster_merge_enabled() && splits < kMaxClusterMerge && tasks * splits * 2 <= info.sm_count &&
+           units / (splits * 2) >= 2 * 8) {
+      splits *= 2;
+    }
+  } else if (splits == 0) {
     // Units (16 tokens) of the longest request, if the caller said; a block wants at least two
     // rounds of its warps' worth so that the ring has something to overlap.
     const long long units = static_cast<long long>(a.max_pages_hint) * (a.page_size / kUnitTokens);

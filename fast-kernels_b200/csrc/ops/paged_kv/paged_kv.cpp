@@ -130,16 +130,7 @@ void shared_prefix_decode_forward(
   tail.page_size = page_size;
   tail.kv_format = kv_format;
   tail.keys_are_rotated = 1;
-  // Without scratch: one block per (request, kv head, 8 query heads), or a cluster of 2 or 4 blocks that
-  // merges through shared memory where there are few and each still has two rounds of its warps to do.
-  const long long tasks = num_kv_heads > 0 ? static_cast<long long>(batch) * num_kv_heads *
-                                                 ((num_q_heads / num_kv_heads + 7) / 8)
-                                           : 0;
-  const long long units = static_cast<long long>(max_tail_pages) * (page_size / 16);
-  tail.splits = 1;
-  while (tail.splits < 4 && tasks * tail.splits * 2 <= 148 && units / (tail.splits * 2) >= 2 * 8) {
-    tail.splits *= 2;
-  }
+  tail.splits = 0;  // without a workspace: what merges through shared memory
   tail.max_pages_hint = max_tail_pages;
   tail.softmax_scale = softmax_scale;
   tail.rope_theta = rope_theta;

@@ -135,7 +135,8 @@ FK_PAGE_DECODE_API int fk_page_decode_forward(const fk_page_decode_args* args);
  * keys_are_rotated the query is turned by the angle that fk_paged_kv_attention turns it by (64-bit fixed point)
  * instead of the fp32 product position * frequency of fk_page_decode_forward. The
  * kernel launched before this one on the stream must be the one that writes the rows; it may write
- * nothing else that this call reads, and must itself have waited for the kernel before it. */
+ * nothing else that this call reads, and must itself have waited for the kernel before it. With splits = 0
+ * and no workspace the call is split as far as it merges without one. */
 typedef struct fk_page_decode_prior {
   const float* rows;         /* 16-byte aligned */
   const int32_t* of_request; /* [batch][2], 8-byte aligned */
