@@ -282,7 +282,7 @@ PYBIND11_MODULE(_native, m) {
     return dql::arc_w4a16_device_status();
   });
 
-  // ---- paged-KV decode attention: the reference's name and keyword arguments, plus three
+  // ---- paged-KV decode attention: the reference's name and keyword arguments, plus four
   // optional ones at the end ------------------------------------------------------------------
   m.def(
       "clustered_page_decode_forward",
@@ -292,14 +292,14 @@ PYBIND11_MODULE(_native, m) {
          int batch, int num_runs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
          int group_tile, int use_clustered_kernel, int cluster_size, int kv_format, int keys_are_rotated,
          float softmax_scale, float rope_theta, ptr_t stream_ptr, int max_pages_hint, int early_descriptors,
-         ptr_t workspace_ptr) {
+         ptr_t workspace_ptr, int exact_turns) {
         py::gil_scoped_release release;
         fast_kernels::clustered_page_decode::clustered_page_decode_forward_hinted(
             query_ptr, key_ptr, value_ptr, key_scales_ptr, value_scales_ptr, run_base_pages_ptr,
             run_page_counts_ptr, run_logical_starts_ptr, run_last_page_lens_ptr, request_run_offsets_ptr,
             seq_lens_ptr, output_ptr, batch, num_runs, num_q_heads, num_kv_heads, head_dim, page_size,
             group_tile, use_clustered_kernel, cluster_size, kv_format, keys_are_rotated, softmax_scale,
-            rope_theta, max_pages_hint, early_descriptors, workspace_ptr, stream_ptr);
+            rope_theta, max_pages_hint, early_descriptors, workspace_ptr, exact_turns, stream_ptr);
       },
       py::arg("query_ptr"), py::arg("key_ptr"), py::arg("value_ptr"), py::arg("key_scales_ptr"),
       py::arg("value_scales_ptr"), py::arg("run_base_pages_ptr"), py::arg("run_page_counts_ptr"),
@@ -309,7 +309,7 @@ PYBIND11_MODULE(_native, m) {
       py::arg("page_size"), py::arg("group_tile"), py::arg("use_clustered_kernel"), py::arg("cluster_size"),
       py::arg("kv_format"), py::arg("keys_are_rotated"), py::arg("softmax_scale"), py::arg("rope_theta"),
       py::arg("stream_ptr"), py::arg("max_pages_hint") = 0, py::arg("early_descriptors") = 0,
-      py::arg("workspace_ptr") = 0);
+      py::arg("workspace_ptr") = 0, py::arg("exact_turns") = 0);
   m.def("page_decode_workspace_bytes", &fast_kernels::clustered_page_decode::page_decode_workspace_bytes, py::arg("batch"),
         py::arg("num_q_heads"), py::arg("num_kv_heads"), py::arg("head_dim"));
   m.def(

@@ -144,8 +144,12 @@ int make_plan(const fk_page_decode_args& a, Plan* plan, bool check_workspace = t
   if (a.splits < 0 || a.splits > kMaxSplits) {
     return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "splits must be in [0, 64]");
   }
-  if ((a.flags & ~FK_PAGE_DECODE_FLAG_EARLY_DESCRIPTORS) != 0) {
+  if ((a.flags & ~(FK_PAGE_DECODE_FLAG_EARLY_DESCRIPTORS | FK_PAGE_DECODE_FLAG_EXACT_TURNS)) != 0) {
     return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "unknown bits in flags");
+  }
+  const bool exact_turns = (a.flags & FK_PAGE_DECODE_FLAG_EXACT_TURNS) != 0;
+  if (exact_turns && a.keys_are_rotated == 0) {
+    return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "exact turns are for keys that are rotated");
   }
   if (a.max_pages_hint < 0) {
     return fail(FK_PAGE_DECODE_ERR_INVALID_ARGUMENT, "max_pages_hint must be non-negative");
@@ -186,7 +190,7 @@ int make_plan(const fk_page_decode_args& a, Plan* plan, bool check_workspace = t
     tile = 4;
   }
   out.variant = Variant{a.head_dim, a.kv_format, a.keys_are_rotated != 0, tile};
-  out.variant.joined = merged;
+  out.variant.joined = merged || exact_turns;
   if (tensor_cores_enabled() && a.keys_are_rotated != 0) {
     // keys that carry their rotation are exact tensor-core operands (8-bit elements convert to
     // bf16 exactly): logits and weighted values as mma.sync, always with the full tile of 8 heads
@@ -406,6 +410,8 @@ int forward(const fk_page_decode_args* args, const fk_page_decode_prior* prior) 
   if (prior != nullptr) {
     params.prior = prior->rows;
     params.prior_of_request = reinterpret_cast<const int2*>(prior->of_request);
+  }
+  if (plan.variant.joined) {
     fk_rope::fill_rope_table(&params.rope, a.head_dim, a.rope_theta);
   }
   params.splits = plan.splits;

@@ -108,7 +108,7 @@ struct JoinedDecodeParams : DecodeParams {
   const int2* prior_of_request;
   // Queries that meet keys with their rotation in them are turned by these angles instead of the fp32 product
   // position * inv_freq: whoever made the prior rows turned the same query by them, and the keys
-  // (paged_kv_append) were. The product is off by 3e-3 radians at position 131071, 5e-2 at 1000000.
+  // (paged_kv_append) were. The product is off by up to 8e-3 radians at position 131071, 6e-2 at 1000000.
   fk_rope::RopeTable rope;
 };
 

@@ -1,6 +1,6 @@
 // Host-side face of the kernel instantiations: one translation unit per (head_dim, page format)
 // holds the kernels of that pair (keys rotated or not x 4 head tiles and the tensor-core form, each
-// plain and joined with prior rows), so that the build compiles them in parallel.
+// plain and with all of JoinedDecodeParams), so that the build compiles them in parallel.
 #pragma once
 
 #include <cuda_runtime.h>

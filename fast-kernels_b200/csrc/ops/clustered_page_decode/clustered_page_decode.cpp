@@ -84,7 +84,7 @@ void clustered_page_decode_forward_hinted(
     int batch, int num_runs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
     int group_tile, int use_clustered_kernel, int cluster_size, int kv_format,
     int keys_are_rotated, float softmax_scale, float rope_theta, int max_pages_hint,
-    int early_descriptors, std::uintptr_t workspace_ptr, std::uintptr_t stream_ptr) {
+    int early_descriptors, std::uintptr_t workspace_ptr, int exact_turns, std::uintptr_t stream_ptr) {
   // the argument rules of the reference's launcher that have no counterpart in the C ABI
   // (clustered_page_decode.cu:1110-1115 there)
   if (cluster_size < 1 || cluster_size > 8) {
@@ -120,7 +120,8 @@ void clustered_page_decode_forward_hinted(
   args.softmax_scale = softmax_scale;
   args.rope_theta = rope_theta;
   args.stream = as<void>(stream_ptr);
-  args.flags = early_descriptors != 0 ? FK_PAGE_DECODE_FLAG_EARLY_DESCRIPTORS : 0;
+  args.flags = (early_descriptors != 0 ? FK_PAGE_DECODE_FLAG_EARLY_DESCRIPTORS : 0) |
+               (exact_turns != 0 ? FK_PAGE_DECODE_FLAG_EXACT_TURNS : 0);
   if (args.splits != 1 && batch > 0 && num_q_heads > 0 && num_kv_heads > 0 && (head_dim == 64 || head_dim == 128)) {
     args.workspace_bytes = fk_page_decode_workspace_bytes(batch, num_q_heads, num_kv_heads, head_dim);
     if (workspace_ptr != 0) {
@@ -153,7 +154,7 @@ void clustered_page_decode_forward(
                                        batch, num_runs, num_q_heads, num_kv_heads, head_dim, page_size, group_tile,
                                        use_clustered_kernel, cluster_size, kv_format, keys_are_rotated,
                                        softmax_scale, rope_theta, /*max_pages_hint=*/0, /*early_descriptors=*/0,
-                                       /*workspace_ptr=*/0, stream_ptr);
+                                       /*workspace_ptr=*/0, /*exact_turns=*/0, stream_ptr);
 }
 
 std::size_t page_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim) {

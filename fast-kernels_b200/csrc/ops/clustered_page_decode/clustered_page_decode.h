@@ -36,8 +36,9 @@ void clustered_page_decode_forward(
 // Additions of this build: the same call with the longest request's page count as a hint (it
 // keeps short requests from being cut into empty pieces), with the caller's word that the
 // kernel before this one in the stream does not write the descriptor arrays (they may then be
-// read while that kernel drains), and with scratch of the caller's for this call alone
-// (page_decode_workspace_bytes, any contents; 0: the stream's); and the device status word.
+// read while that kernel drains), with scratch of the caller's for this call alone
+// (page_decode_workspace_bytes, any contents; 0: the stream's), and with the query's angle in 64-bit
+// fixed point (`exact_turns`, for keys that are rotated); and the device status word.
 void clustered_page_decode_forward_hinted(
     std::uintptr_t query_ptr, std::uintptr_t key_ptr, std::uintptr_t value_ptr,
     std::uintptr_t key_scales_ptr, std::uintptr_t value_scales_ptr,
@@ -47,7 +48,7 @@ void clustered_page_decode_forward_hinted(
     int batch, int num_runs, int num_q_heads, int num_kv_heads, int head_dim, int page_size,
     int group_tile, int use_clustered_kernel, int cluster_size, int kv_format,
     int keys_are_rotated, float softmax_scale, float rope_theta, int max_pages_hint,
-    int early_descriptors, std::uintptr_t workspace_ptr, std::uintptr_t stream_ptr);
+    int early_descriptors, std::uintptr_t workspace_ptr, int exact_turns, std::uintptr_t stream_ptr);
 std::size_t page_decode_workspace_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim);
 int page_decode_device_status();
 

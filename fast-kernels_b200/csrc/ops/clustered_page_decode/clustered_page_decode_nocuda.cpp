@@ -16,7 +16,7 @@ void clustered_page_decode_forward(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, 
   unavailable();
 }
 void clustered_page_decode_forward_hinted(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, int, int, int, int,
-                                          int, int, int, int, int, int, int, float, float, int, int, ptr, ptr) {
+                                          int, int, int, int, int, int, int, float, float, int, int, ptr, int, ptr) {
   unavailable();
 }
 std::size_t page_decode_workspace_bytes(int, int, int, int) { unavailable(); }

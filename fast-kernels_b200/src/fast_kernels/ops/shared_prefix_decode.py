@@ -46,6 +46,11 @@ _PLANS: OrderedDict = OrderedDict()
 # 252 MB 33.2 / 49.9. Not the bytes alone count: 4096 shared tokens pay from 25 to 60 MB on, and few heads with many
 # requests later (2 heads of 128 x 8, 64 requests, bf16: 66 MB 26.0 / 20.1).
 DEFAULT_MIN_SAVED_BYTES = 64 << 20
+# From this length on the plain decode's angle, an fp32 product of position and frequency, is not good enough for keys whose
+# own angle is exact (paged_kv_append): off by up to 2e-3 radians here (logits by 1e-4 on average, their outputs' rounding is
+# 2e-3), and growing with the position. Shorter requests that share nothing are turned by it all the same, and so have the bits
+# of clustered_page_decode.
+FAR_TOKENS = 32768
 # Shared runs shorter than this stay with the requests (or with longer runs further down).
 MIN_RUN_TOKENS = 128
 
@@ -68,6 +73,7 @@ class SharedPrefixDecodePlan:
     items_cpu: Any       # int32 [items, 8]
     of_request_cpu: Any  # int32 [batch, 2]: first partial result, partial results
     tail_plan: ClusteredPageDecodePlan  # what every request has to itself (all of it where nothing is shared)
+    far: bool  # some request is longer than FAR_TOKENS
     _device_cache: dict[int, Any] = field(default_factory=dict, repr=False)
 
     @property
@@ -210,7 +216,8 @@ def _build(table: np.ndarray, lens: np.ndarray, num_q_heads: int, num_kv_heads: 
         estimated_saved_hbm_bytes=saved, num_partials=int(partials.sum()), largest_page=int(used.max()) if used.size else -1,
         runs=[(first, end, tuple(sorted(order[low:high].tolist()))) for first, end, low, high in runs],
         page_ids_cpu=torch.from_numpy(page_ids.astype(np.int32)), vectors_cpu=torch.from_numpy(vectors.astype(np.int32)),
-        items_cpu=torch.from_numpy(items), of_request_cpu=torch.from_numpy(of_request.astype(np.int32)), tail_plan=tail_plan)
+        items_cpu=torch.from_numpy(items), of_request_cpu=torch.from_numpy(of_request.astype(np.int32)), tail_plan=tail_plan,
+        far=int(lens.max()) > FAR_TOKENS)
 
 
 def shared_prefix_decode(
@@ -250,7 +257,7 @@ def shared_prefix_decode(
             _paged.keep_for_graphs(plan)
         tables = plan.device_tables(device, stream)
         tail = plan.tail_plan
-        if not plan.runs:  # the launch that clustered_page_decode makes
+        if not plan.runs:  # the launch that clustered_page_decode makes, except for the angle of far queries
             # (it may split long requests through scratch: the stream's, or, since graphs that were captured on one stream
             # may be replayed at the same time, a captured call's own)
             scratch = None
@@ -264,7 +271,8 @@ def shared_prefix_decode(
                 tables["run_last_page_lens"], tables["request_run_offsets"], tables["seq_lens"], output.data_ptr(), plan.batch,
                 tail.num_runs, plan.num_q_heads, plan.num_kv_heads, plan.head_dim, plan.page_size, tail.group_tile, int(not direct),
                 1 if direct else max(2, tail.cluster_size), _layout_id(plan.kv_layout), int(cache.keys_are_rotated), float(scale),
-                float(rope_theta), stream, max_pages_hint=tail.max_pages, early_descriptors=1, workspace_ptr=_paged.address(scratch))
+                float(rope_theta), stream, max_pages_hint=tail.max_pages, early_descriptors=1, workspace_ptr=_paged.address(scratch),
+                exact_turns=int(plan.far))
             return output
         partials = torch.empty((plan.num_partials, plan.num_q_heads, plan.head_dim + 4), dtype=torch.float32, device=device)
         native.shared_prefix_decode_forward(

@@ -21,6 +21,7 @@ KV_BF16 = 0
 KV_FP8_E4M3 = 1
 KV_INT8 = 2
 FLAG_EARLY_DESCRIPTORS = 1
+FLAG_EXACT_TURNS = 2
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libfk_page_decode.so"
 

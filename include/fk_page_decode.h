@@ -65,6 +65,10 @@ extern "C" {
  * they come from the host -- and the kernel reads and sorts them before it waits. Queries, pages,
  * scales and outputs are never touched early. */
 #define FK_PAGE_DECODE_FLAG_EARLY_DESCRIPTORS 1
+/* The query is turned by the 64-bit fixed-point angle that fk_paged_kv_append turns keys by and fk_paged_kv_attention its
+ * queries, instead of the fp32 product position * frequency (off by up to 2e-3 radians at position 32768, 8e-3 at 131071,
+ * 6e-2 at 1000000). Only with keys_are_rotated. */
+#define FK_PAGE_DECODE_FLAG_EXACT_TURNS 2
 
 typedef struct fk_page_decode_args {
   const void* query;

@@ -105,3 +105,42 @@ def test_a_shared_decode_far_out_turns_its_queries_by_one_angle(layout, dim) -> 
         assert float((off / bound).max()) <= 1.0, float((off / bound).max())
     torch.cuda.synchronize()
     assert native_module().paged_kv_device_status() == 0 and native_module().page_decode_device_status() == 0
+
+
+@pytest.mark.parametrize("layout", ["bf16_kv", "int8_kv"])
+def test_a_far_decode_that_shares_nothing_is_turned_by_the_same_angle(layout) -> None:
+    """As above with one request, in a graph too. No part of it is rounded to 16 bits but for the row: weights and query are
+    16-bit heads and remainders."""
+    ps, theta, before_own, own, dim = 32, 10000.0, 31_250, 25, 128
+    table = np.zeros((1, before_own + 1), dtype=np.int32)
+    table[0, -1] = 1
+    length = before_own * ps + own
+    cache = random_cache(layout=layout, pages=2, heads=2, page_size=ps, dim=dim, table=table, lens=[length], theta=theta, seed=1)
+    cache.key_pages[0] = 0
+    query = torch.randn((1, 8, dim), generator=torch.Generator().manual_seed(2)).to(torch.bfloat16).cuda()
+    plan = ops.plan_shared_prefix_decode(page_table=cache.page_table, seq_lens=cache.seq_lens, num_q_heads=8, num_kv_heads=2, head_dim=dim,
+                                         page_size=ps, kv_layout=layout, use_cache=False)
+    assert plan.runs == []
+    scale = 8.0 / math.sqrt(dim)
+    got = ops.shared_prefix_decode(query, cache, plan=plan, softmax_scale=scale)
+    graph, again = torch.cuda.CUDAGraph(), torch.empty_like(got)
+    with torch.cuda.graph(graph):
+        ops.shared_prefix_decode(query, cache, plan=plan, softmax_scale=scale, output=again)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got.view(torch.int16), again.view(torch.int16))
+    keys, values = cache_values(cache)
+    turned = rotate64(query.cpu(), [length - 1], theta)[0].reshape(2, 4, dim)
+    k, v = keys[1, :, :own], values[1, :, :own]
+    logits = torch.einsum("hgd,htd->hgt", turned, k) * scale
+    top = logits.amax(dim=-1, keepdim=True)
+    weights, before = torch.exp(logits - top), torch.exp(-top) * before_own
+    total = weights.sum(dim=-1, keepdim=True) + before * ps
+    want = (torch.einsum("hgt,htd->hgd", weights, v) + before * values[0].sum(dim=1)[:, None]) / total
+    a = (torch.einsum("hgt,htd->hgd", weights, v.abs()) + before * values[0].abs().sum(dim=1)[:, None]) / total
+    d = 2.0**-16 * scale * torch.einsum("hgd,htd->hgt", turned.abs(), k.abs()).amax(dim=-1, keepdim=True)
+    # (a million fp32 weights of about e^-top each, added one after the other in blocks: 2^-12 of their share at most)
+    bound = 2.0**-8 * want.abs() + (2.0**-16 + 2.2 * d) * a + 2.0**-12 * before * values[0].abs().sum(dim=1)[:, None] / total
+    off = (got.double().cpu().reshape(2, 4, dim) - want).abs()
+    assert float((off / bound).max()) <= 1.0, float((off / bound).max())
+    assert native_module().page_decode_device_status() == 0
