@@ -36,7 +36,10 @@
 // tile of 128-dimensional rows is two such halves. bf16 pages are copied there by TMA, one box of
 // page_size rows per page and half. 8-bit pages are copied as they are and converted by four warps to
 // fp16, exactly for the 64-dim block with the page's (keys) or token's (values) larger scale, the other
-// block times the ratio of the two scales. The larger scales stay fp32: the page's goes on the logits,
+// block times the ratio of the two scales. Where there are two blocks both are multiplied by 2^7 (e4m3's 448
+// becomes 57344), which leaves the smaller one all 11 bits down to a ratio of 2^-21, and those of a bf16 result down
+// to 2^-24; it comes off in fp32, with the page's factor and behind the last product.
+// The larger scales stay fp32: the page's goes on the logits,
 // the token's on the probability before it is rounded. (Values in bf16 with bf16 probabilities took five
 // times the conversion's instructions, and their two roundings made the error 1.5 times the output's own.)
 //
@@ -221,9 +224,11 @@ __device__ __forceinline__ float largest_of(const uint32_t* r) {
   return max3(a, b, max3(a, __uint_as_float(r[N - 2]), __uint_as_float(r[N - 1])));
 }
 
-// Two copies of mine / larger in fp16 (exactly 1 for the block that has the larger scale).
+// Two copies of mine / larger in fp16, times 2^7 (exactly that for the block that has the larger scale).
+constexpr float kRatioPower = 128.0f;
+constexpr float kRatioLog2 = 7.0f;
 __device__ __forceinline__ uint32_t scale_ratio(float mine, float larger) {
-  const __half2 ratio = __float2half2_rn(larger > 0.0f ? __fdividef(mine, larger) : 0.0f);
+  const __half2 ratio = __float2half2_rn(larger > 0.0f ? __fdividef(mine, larger) * kRatioPower : 0.0f);
   return *reinterpret_cast<const uint32_t*>(&ratio);
 }
 __device__ __forceinline__ uint32_t mul_half2(uint32_t a, uint32_t b) {
@@ -670,7 +675,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
       const bool direct = item.partial < 0;
       const bool write_row = r < rows && vec.x >= 0 && vec.x < p.num_rows &&
                              (direct || (item.partial < vec.w && vec.z >= 0 && vec.z + item.partial < p.num_partials));
-      const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+      constexpr float kPower = QUANT && kBlocks == 2 ? kRatioPower : 1.0f;  // what the values were multiplied by
+      constexpr float kPowerLog2 = QUANT && kBlocks == 2 ? kRatioLog2 : 0.0f;
+      const float inv = l == 0.0f ? 0.0f : (1.0f / kPower) / l;
       constexpr uint32_t kRowBytes = (D + 4) * 4;  // 16 bytes off a multiple of 128: lanes take turns at the banks
       const uint32_t staged = base + r * kRowBytes;
 #pragma unroll
@@ -702,7 +709,8 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
         }
       }
       if (!direct) {
-        sts128(staged + D * 4, make_uint4(__float_as_uint(m), __float_as_uint(l), 0u, 0u));
+        // (the values keep their power: denominator and maximum are brought to it)
+        sts128(staged + D * 4, make_uint4(__float_as_uint(m - kPowerLog2), __float_as_uint(l * kPower), 0u, 0u));
       }
       proxy_fence_async();
       if (write_row) {
@@ -956,7 +964,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           const float2 s = *reinterpret_cast<const float2*>(smem + L::kRawKeyScales + raw_slot * 64 + page * 8);
           const float larger = fmaxf(s.x, s.y);
           if ((t & (p.page_size - 1)) == 0) {
-            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + page] = larger;
+            reinterpret_cast<float*>(smem + L::kKeyFactors)[(j % kFactorRing) * 8 + page] = kBlocks == 2 ? larger * (1.0f / kRatioPower) : larger;
           }
           if constexpr (kBlocks == 2) {
             ratios[t] = make_uint2(scale_ratio(s.x, larger), scale_ratio(s.y, larger));
