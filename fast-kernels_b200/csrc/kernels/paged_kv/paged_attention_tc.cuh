@@ -247,6 +247,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
   // How far a row's largest probability (weight) may be above 1, as a power of two, before O is rescaled:
   // 8-bit pages, fp16 weights: below 2^16; bf16 has the range, and O should not lose it.
   constexpr float kGrowth = QUANT ? 15.0f : 8.0f;
+  constexpr float kHeadroom = 7.0f;
   constexpr uint32_t kScoresDesc = instruction_desc(!QUANT, kTileTokens, false);
   constexpr uint32_t kValuesDesc = instruction_desc(!QUANT, D, true);
   extern __shared__ __align__(16) uint8_t raw_smem[];
@@ -480,7 +481,8 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
     const float power = QUANT && count > 0 ? row_power[r] : 1.0f;
     // `m` is what probabilities are relative to, 2^(logit - m). bf16 pages: the largest logit (kept lazily).
     // 8-bit pages: the largest logit + log2 of the token's value scale, that is the heaviest weight
-    // (probability times scale), which is what has to stay within fp16.
+    // (probability times scale), which is what has to stay within fp16, less kHeadroom: the heaviest weight is 2^kHeadroom
+    // to begin with and may grow to 2^kGrowth, so that one of 2^-21 of it still has all its bits.
     float m = -INFINITY, l = 0.0f;
     bool ok = true;
     for (int j = 0; j < tiles[x]; ++j) {
@@ -567,6 +569,7 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
               top = max3(top, max3(a, b, e), g);
             }
           }
+          top -= kHeadroom;
         } else {
           top = m;
         }
@@ -979,8 +982,9 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           }
           float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
           factors[0] = t < valid ? larger : 0.0f;
-          // (a scale of 0 must not leave a tile without a finite heaviest weight)
-          const float log = t < valid ? __log2f(fmaxf(larger, 1e-30f)) : -INFINITY;
+          // (a scale of 0 must not leave a tile without a finite heaviest weight, nor one near it make the sum of
+          // probabilities, 2^-log each at most, overflow)
+          const float log = t < valid ? __log2f(fmaxf(larger, 1e-28f)) : -INFINITY;
           factors[kFactorRing * kTileTokens] = log;
           float most = log;
 #pragma unroll

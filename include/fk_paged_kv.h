@@ -108,8 +108,8 @@ typedef struct fk_paged_kv_append_args {
  * exact power of two; keys and values are fp16 numbers, exact in the 64-dim block that has the page's
  * (token's) larger scale, the other block's times the ratio of the two scales (off by up to 2^-10 of itself down
  * to a ratio of 2^-21, by 2^-8 at 2^-24, and lost at 2^-32); a probability times its
- * token's larger value scale is rounded to fp16 relative to the row's heaviest, so that one below 2^-14
- * of it is off by up to 2^-25 of it. A non-finite key or value of a token that counts may reach every
+ * token's larger value scale is rounded to fp16 relative to the row's heaviest, so that one below 2^-21
+ * of it is off by up to 2^-32 of it. A non-finite key or value of a token that counts may reach every
  * vector of an item; what lies behind a request's last token is never used. Results do not depend on
  * timing. */
 #define FK_PAGED_KV_ITEM_ROWS 256

@@ -77,3 +77,17 @@ def test_the_block_with_the_smaller_scales_keeps_its_bits(layout, exponent, larg
     bound = 2.0**-8 + 2.0**-11 + 17 / 16 * max(2.0**-25 / (128 * ratio), 2.0**-11) + 2.0**-12
     assert bound < 2.0**-6.9
     _assert_means(cache, bound)
+
+
+@pytest.mark.parametrize("layout", ["fp8_kv", "int8_kv"])
+@pytest.mark.parametrize("exponent", [-18, -20, -22])
+def test_a_token_with_one_large_block_takes_no_bits_from_the_others(layout, exponent) -> None:
+    """Every other token has its first block's scale far above all others; in the second block all tokens count alike. A
+    weight of r = 1.35 * 2^exponent of the heaviest, which is 2^7 or more, is off by up to 2^-25 / (2^7 r), or 2^-11, and so are the
+    heavy tokens' ratio and (as above) its products; with the row and the sums as above."""
+    cache = _cache(layout)
+    ratio = 1.35 * 2.0**exponent
+    cache.value_scales[:] = 0.75 * ratio
+    cache.value_scales[:, :, ::2, 0] = 0.75
+    small = max(2.0**-25 / (128 * ratio), 2.0**-11)
+    _assert_means(cache, 2.0**-8 + 2.0**-11 + (2 + 1 / 16) * small + 2.0**-12)
