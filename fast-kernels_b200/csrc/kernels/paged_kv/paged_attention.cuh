@@ -39,12 +39,13 @@ __device__ __forceinline__ Item load_item(const AttentionParams& p, int index) {
   const int4 a = p.items[2 * index], b = p.items[2 * index + 1];
   return Item{a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
-// What the caller's tables may not make the kernels do: leave the arrays.
+// What the caller's tables may not make the kernels do: leave the arrays, or count past 31 bits (the kernel counts
+// whole tiles of up to 128 tokens).
 __device__ __forceinline__ bool item_fits(const AttentionParams& p, const Item& item) {
   return item.first_vector >= 0 && item.vectors > 0 && item.vectors <= FK_PAGED_KV_ITEM_ROWS / p.group &&
          item.first_vector <= p.num_vectors - item.vectors && item.kv_head >= 0 && item.kv_head < p.num_kv_heads &&
          item.entry >= 0 && item.first_token >= 0 && item.first_token % p.page_size == 0 && item.partial >= -1 &&
-         item.end_token >= item.first_token &&
+         item.end_token >= item.first_token && item.end_token <= FK_PAGED_KV_MAX_TOKENS &&
          static_cast<long long>(item.entry) + (static_cast<long long>(item.end_token) + p.page_size - 1) / p.page_size <=
              p.num_page_ids;
 }

@@ -71,6 +71,12 @@ def table_and_lengths(page_table: Any, **lengths: Any) -> list[np.ndarray]:
     return out
 
 
+def require_countable(lens: np.ndarray) -> None:
+    """The attention kernel counts a request's tokens in 32 bits, a tile at a time (FK_PAGED_KV_MAX_TOKENS)."""
+    if lens.size and int(lens.max()) > (1 << 31) - 128:
+        raise ValueError("seq_lens must be at most 2^31 - 128")
+
+
 def require_pages(table: np.ndarray, request: np.ndarray, slot: np.ndarray) -> np.ndarray:
     """Physical pages of (request, logical page) pairs; every one must be in the table."""
     if slot.size and int(slot.max()) >= table.shape[1]:

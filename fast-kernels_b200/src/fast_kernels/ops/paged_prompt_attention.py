@@ -73,6 +73,7 @@ def plan_paged_prompt_attention(
     if num_q_heads // num_kv_heads > _paged_items.ITEM_ROWS:
         raise ValueError(f"at most {_paged_items.ITEM_ROWS} query heads per kv head")
     table, lens, new = _paged.table_and_lengths(page_table, seq_lens=seq_lens, query_lens=query_lens)
+    _paged.require_countable(lens)
     if lens.size and bool((new > lens).any()):
         raise ValueError("query_lens must not exceed seq_lens")
     made_from = (table, lens, new, num_q_heads, num_kv_heads, head_dim, page_size, layout)
@@ -84,6 +85,8 @@ def _build(table: np.ndarray, lens: np.ndarray, new: np.ndarray, num_q_heads: in
     torch = _torch()
     lens = np.where(new > 0, lens, 0)  # a request without queries needs no pages
     pages = -(-lens // page_size)
+    if pages.size and int(pages.max()) > table.shape[1]:
+        raise ValueError("page_table has fewer columns than the tokens need")
     request = np.repeat(np.arange(len(lens)), pages)
     entries = np.cumsum(pages) - pages
     page_ids = _paged.require_pages(table, request, np.arange(int(pages.sum())) - entries[request])

@@ -141,6 +141,7 @@ def plan_shared_prefix_decode(
     table, lens = _paged.table_and_lengths(page_table, seq_lens=seq_lens)
     if lens.size == 0:
         raise ValueError("the batch must not be empty")
+    _paged.require_countable(lens)
     made_from = (table, lens, num_q_heads, num_kv_heads, head_dim, page_size, layout, min_saved_bytes)
     return _paged.remembered(_PLANS, made_from, lambda: _build(*made_from), use_cache)
 
@@ -150,9 +151,9 @@ def _build(table: np.ndarray, lens: np.ndarray, num_q_heads: int, num_kv_heads: 
     torch = _torch()
     batch = len(lens)
     pages = -(-lens // page_size)
-    slots = np.arange(int(pages.max()))
     if int(pages.max()) > table.shape[1]:
         raise ValueError("page_table has fewer columns than the tokens need")
+    slots = np.arange(int(pages.max()))
     table = table[:, : len(slots)]
     used = table[slots < pages[:, None]]
     if used.size and int(used.min()) < 0:

@@ -101,7 +101,8 @@ typedef struct fk_paged_kv_append_args {
  * kernel adds the partial results of every vector that has some, in order, into `output`; without it
  * the caller hands them to fk_page_decode_forward_merged.
  *
- * The positions of a causal item's vectors ascend. An item that does not fit the arrays is left out.
+ * The positions of a causal item's vectors ascend. An item that does not fit the arrays, or ends behind
+ * FK_PAGED_KV_MAX_TOKENS, is left out.
  *
  * Rounding. Logits, maxima, denominators and weighted values are fp32. bf16 pages: the turned query and the
  * probabilities are rounded to bf16 once. 8-bit pages: the turned query is rounded to fp16 behind an
@@ -113,6 +114,7 @@ typedef struct fk_paged_kv_append_args {
  * vector of an item; what lies behind a request's last token is never used. Results do not depend on
  * timing. */
 #define FK_PAGED_KV_ITEM_ROWS 256
+#define FK_PAGED_KV_MAX_TOKENS (0x7fffffff - 127) /* of an item's end token */
 typedef struct fk_paged_kv_attention_args {
   const void* query; /* bf16 rows [rows][num_q_heads][head_dim], strides below, 16-byte aligned rows */
   int64_t query_row_stride; /* in elements, multiples of 8 */
