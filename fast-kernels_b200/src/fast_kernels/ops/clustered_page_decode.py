@@ -611,6 +611,8 @@ def materialize_reference_dense_kv(cache: PagedKVCache) -> tuple[Any, Any]:
     """[batch, kv_heads, max_seq_len, head_dim] keys and values gathered back through the page table
     from the unquantised pages."""
     torch = _torch()
+    if cache.reference_key_pages is None or cache.reference_value_pages is None:
+        raise ValueError("the cache has no unquantised pages")
     batch = int(cache.page_table.shape[0])
     max_len = int(cache.seq_lens.max().item())
     pages = cache.reference_key_pages

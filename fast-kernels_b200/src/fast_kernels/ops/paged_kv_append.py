@@ -14,8 +14,9 @@ says:
   already become ``round(q s / s')``. A prompt appended at once to fresh pages gives the scales that
   ``quantize_paged_kv_int8`` / ``_fp8`` compute.
 
-The pages are written in place. ``reference_key_pages`` / ``reference_value_pages`` are not: a cache
-that grows by this operator has none for 8-bit layouts (``empty_paged_kv``). A page that two requests
+The pages are written in place. ``reference_key_pages`` / ``reference_value_pages`` are not: the cache that
+is returned has them only where they are the pages themselves (bf16), not where they would lack the new
+tokens. A page that two requests
 share is the caller's to copy before one of them writes to it; two requests that would write to the
 same page are refused.
 """
@@ -174,4 +175,8 @@ def paged_kv_append(
                 _layout_id(plan.kv_layout), int(cache.keys_are_rotated),
                 float(cache.key_rope_theta) if cache.keys_are_rotated else 1.0, stream)
     # (a copy: the plan may be used again, and the caller may write to the cache's lengths)
-    return dataclasses.replace(cache, seq_lens=plan.seq_lens_after_cpu.clone())
+    changes = {"seq_lens": plan.seq_lens_after_cpu.clone()}
+    for name in ("key_pages", "value_pages"):
+        if plan.num_tokens and getattr(cache, f"reference_{name}") is not getattr(cache, name):
+            changes[f"reference_{name}"] = None
+    return dataclasses.replace(cache, **changes)
