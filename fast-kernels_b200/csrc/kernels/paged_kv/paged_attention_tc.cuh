@@ -43,10 +43,16 @@
 // the token's on the probability before it is rounded. (Values in bf16 with bf16 probabilities took five
 // times the conversion's instructions, and their two roundings made the error 1.5 times the output's own.)
 //
+// bf16 pages: query and probabilities are bf16 because both operands of a product have one type, and are rounded
+// once. Each of the two roundings is as large as the output's own: 2.5e-3 to 2.9e-3 in the 2-norm for 1.65e-3. A
+// remainder of the query as a second operand would take half as much tensor work again and 64 KB of shared memory for
+// one of them, a remainder of the probabilities as much again and a second conversion in the softmax.
+//
 // What it measures: 8192 tokens, 32 heads over 8 of 128, bf16, causal: 574 us, 958 TFLOP/s, 59 % of the
 // measured bf16 peak: a token tile takes 3350 clocks where the products need 2050. 512 tokens behind 32768
-// in fp8 pages, 32 heads over 4: 427 us, 650 TFLOP/s, 5500 clocks a tile: bound by the conversion, in the
-// issue slots of the softmax warps, and the chain behind it.
+// in fp8 pages, 32 heads over 4: 418 us, 661 TFLOP/s, 5400 clocks a tile: bound by the conversion, in the
+// issue slots of the softmax warps, and the chain behind it. (Waits with one verdict a warp, and so without
+// divergence behind them, were worth 10 of 427 us.)
 // Tried and slower: steps of 64 tokens with two buffers of logits per row tile (N = 64 costs the tensor
 // core as much as N = 128 when both operands come from shared memory: 748 us), four more converting warps
 // (fewer registers for the softmax: 602 us for 477), a quarter or half of the exponentials as polynomials

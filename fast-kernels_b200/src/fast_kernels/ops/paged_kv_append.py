@@ -145,7 +145,7 @@ def paged_kv_append(
     """Writes `keys` and `values` (bf16, [tokens, kv_heads, head_dim], the requests' new tokens one request
     after the other; views into a fused projection's rows will do) into the cache's pages. Either
     `append_lens` or a `plan` says how many tokens each request gets. Returns the cache with the new
-    `seq_lens`; its pages are the same tensors."""
+    `seq_lens`, as int32 on the CPU wherever the cache had them (plans are made there); its pages are the same tensors."""
     native = _paged.backend()
     found = plan is None
     if plan is None:

@@ -12,6 +12,13 @@ Grouped-query heads share a kernel tile, so a page is read once for all of them.
 work into items (up to 256 query rows of one kv head over a range of tokens) that fill the device, and
 cuts long ranges in pieces whose partial results a second kernel adds in order: results do not depend
 on timing. Inference only: there is no backward pass.
+
+bf16 pages: the turned query and the weights are rounded to bf16 once (the tensor cores take both operands in
+one type), the row is off by 2.5e-3 to 2.9e-3 in the 2-norm where its own rounding is 1.7e-3. 8-bit pages: fp16, the
+row's own rounding, as long as the scales of a token's (keys: a page's) two 64-dim blocks are within 2^24 of each other.
+
+A bounded wait inside the kernel that gives up leaves the call's output invalid and raises nothing:
+``fast_kernels.native.native_module().paged_kv_device_status()`` is 0 while none has.
 """
 
 from __future__ import annotations

@@ -14,6 +14,16 @@ over the runs that a request takes part in and its own tokens, maxima and sums i
 order. Where sharing would not pay (``estimated_saved_hbm_bytes`` below what the second kernel costs)
 the plan is the plain decode.
 
+Over shared runs of bf16 pages the turned query and the weights are rounded to bf16 once (the tensor cores
+take both operands in one type): a row is off by 2.9e-3 in the 2-norm where the plain decode, which carries
+both as 16-bit heads and remainders, has the output's own rounding, 1.7e-3. A request's row is so less exact when its batch
+shares than when it does not; ``min_saved_bytes`` beyond any saving keeps the plan plain. 8-bit pages have
+fp16 weights and stay at the output's rounding.
+
+A bounded wait inside a kernel that gives up leaves the call's output invalid and raises nothing:
+``fast_kernels.native.native_module()`` has ``paged_kv_device_status()`` and ``page_decode_device_status()``, 0 while
+none has.
+
 ``prefix_union_decode`` keeps the contract of the op of that name, which on this device computes every
 request by itself.
 """
@@ -131,7 +141,8 @@ def plan_shared_prefix_decode(
     min_saved_bytes: int = DEFAULT_MIN_SAVED_BYTES,
     use_cache: bool = True,
 ) -> SharedPrefixDecodePlan:
-    """`min_saved_bytes` is what sharing must save of a call's traffic before the plan shares at all (0: always)."""
+    """`min_saved_bytes` is what sharing must save of a call's traffic before the plan shares at all (0: always). The plan is
+    the caller's to keep as long as graphs that were captured with it."""
     layout = _paged.require_geometry(num_kv_heads=num_kv_heads, head_dim=head_dim, page_size=page_size, kv_layout=kv_layout,
                                      num_q_heads=num_q_heads)
     if num_q_heads // num_kv_heads > _paged_items.ITEM_ROWS:
@@ -231,7 +242,9 @@ def shared_prefix_decode(
     rope_theta: float = 10000.0,
 ) -> Any:
     """`query` is bf16 [batch, q_heads, head_dim], contiguous, not yet turned by its positions; request b's token is the
-    last of its `seq_lens[b]`. The cache's keys are turned ahead of time (`key_rope_theta`)."""
+    last of its `seq_lens[b]`. The cache's keys are turned ahead of time (`key_rope_theta`). Requests that share pages, and
+    batches with one beyond `FAR_TOKENS`, have their queries turned by exact angles (as `paged_kv_append` turns keys);
+    others by those of `clustered_page_decode`, products in fp32."""
     torch = _torch()
     native = _paged.backend()
     if not isinstance(query, torch.Tensor):
