@@ -989,8 +989,8 @@ __global__ void __launch_bounds__(TcLayout<D, KV>::kThreads, 1)
           float* factors = reinterpret_cast<float*>(smem + L::kValueFactors) + (j % kFactorRing) * kTileTokens + t;
           factors[0] = t < valid ? larger : 0.0f;
           // (a scale of 0 must not leave a tile without a finite heaviest weight, nor one near it make the sum of
-          // probabilities, 2^-log each at most, overflow)
-          const float log = t < valid ? __log2f(fmaxf(larger, 1e-28f)) : -INFINITY;
+          // probabilities, 2^(kGrowth - log) each at most, overflow; scales from 5e-31 on have all their weights' bits)
+          const float log = t < valid ? __log2f(fmaxf(larger, 1e-24f)) : -INFINITY;
           factors[kFactorRing * kTileTokens] = log;
           float most = log;
 #pragma unroll
