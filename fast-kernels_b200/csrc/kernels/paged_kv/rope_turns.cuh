@@ -37,9 +37,9 @@ __device__ __forceinline__ float2 rope_cos_sin(uint64_t turns_per_position, int 
   const float half_turns = static_cast<float>(static_cast<int32_t>(turns - (quarters << 30))) * 0x1p-31f;  // in [-1/4, 1/4]
   float sn, cs;
   sincospif(half_turns, &sn, &cs);
-  const float c = (quarters & 1u) != 0 ? -sn : cs;
-  const float s = (quarters & 1u) != 0 ? cs : sn;
-  return (quarters & 2u) != 0 ? make_float2(-c, -s) : make_float2(c, s);
+  const uint32_t c = __float_as_uint((quarters & 1u) != 0 ? sn : cs);
+  const uint32_t s = __float_as_uint((quarters & 1u) != 0 ? cs : sn);
+  return make_float2(__uint_as_float(c ^ (((quarters + 1u) & 2u) << 30)), __uint_as_float(s ^ ((quarters & 2u) << 30)));
 }
 
 // The same, off by up to 2^-20.5: for a query that is rounded to 16 bits behind it.

@@ -175,8 +175,8 @@ def paged_kv_append(
                 _layout_id(plan.kv_layout), int(cache.keys_are_rotated),
                 float(cache.key_rope_theta) if cache.keys_are_rotated else 1.0, stream)
     # (a copy: the plan may be used again, and the caller may write to the cache's lengths)
-    changes = {"seq_lens": plan.seq_lens_after_cpu.clone()}
-    for name in ("key_pages", "value_pages"):
-        if plan.num_tokens and getattr(cache, f"reference_{name}") is not getattr(cache, name):
-            changes[f"reference_{name}"] = None
-    return dataclasses.replace(cache, **changes)
+    lens = plan.seq_lens_after_cpu.clone()
+    kept = cache.reference_key_pages, cache.reference_value_pages
+    if plan.num_tokens and (kept[0] is not None and kept[0] is not cache.key_pages or kept[1] is not None and kept[1] is not cache.value_pages):
+        return dataclasses.replace(cache, seq_lens=lens, reference_key_pages=None, reference_value_pages=None)
+    return dataclasses.replace(cache, seq_lens=lens)
