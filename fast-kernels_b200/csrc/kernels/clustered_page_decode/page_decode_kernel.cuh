@@ -667,7 +667,8 @@ __global__ void __launch_bounds__((MMA ? kMaxWarpsNarrow : max_warps_for(GT)) * 
     // ---- this warp's units ----
     for (int i = warp; i < in_round && !failed; i += warps, ++iteration) {
       const int stage = iteration % stages;
-      if (!mbar_wait_bounded(my_bars + stage * 8, (iteration / stages) & 1)) {
+      // (one verdict for the warp: what follows needs all its lanes)
+      if (!__all_sync(0xffffffffu, mbar_wait_bounded(my_bars + stage * 8, (iteration / stages) & 1))) {
         failed = true;
         if (lane == 0) {
           atomicExch(p.status, kStatusCopyWaitTimeout);

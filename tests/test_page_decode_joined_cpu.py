@@ -28,3 +28,13 @@ def test_the_plain_instances_have_nothing_of_the_join() -> None:
             elif open_blocks:  # (the namespace's own brace closes last)
                 open_blocks.pop()
     assert uses >= 3
+
+
+def test_a_warp_gives_up_a_wait_as_a_whole() -> None:
+    """The limit of a unit's wait runs out lane by lane, and what follows it are shuffles and products of whole warps. (The
+    waits behind the loop only let copies land: nothing hangs on their verdicts.)"""
+    source = re.sub(r"//.*", "", (KERNELS / "page_decode_kernel.cuh").read_text())
+    kernel = source[source.index("page_decode_kernel("):]
+    waits = re.findall(r"([^\n;{}]*)mbar_wait_bounded\(", kernel)
+    assert len(waits) == 2
+    assert "if (!__all_sync(0xffffffffu, " in waits[0] and "(void)" in waits[1]
